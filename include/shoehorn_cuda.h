@@ -177,6 +177,66 @@ int shc_encode_rows_noalloc(uint32_t ggml_type, uint32_t src_type, const void *s
                             const float *imatrix, int64_t imatrix_len, int64_t rows_per_mat, int64_t row0,
                             uint8_t *dst, void *stream);
 
+/* ---------------------------------------------------------------- 8-bit blocks
+ *
+ * Block-scaled 8-bit codes and the products that multiply them, for programs
+ * that run what the encoders above prepare.  No counterpart in the reference
+ * (it leaves inference to llama.cpp).
+ *
+ * Format: E4M3 codes with one f32 scale for each block, value = code * scale.
+ * A block is 128 consecutive columns of one row (block_rows 1, for
+ * activations and gradients) or a tile of 128 rows x 128 columns (block_rows
+ * 128, for weights); the last block of a row or of a matrix's rows may be
+ * part empty.
+ *
+ *   top   = max(max |x| over the block's finite elements, 448 * 2^-126)
+ *   scale = top / 448           code = e4m3(x * (448 / top)), ties to even
+ *
+ * NaN and infinite elements become the NaN code 0x7F and do not count in top.
+ * Matrices of codes start on 16-byte boundaries, and their row (and matrix)
+ * strides are multiples of 16 bytes; bytes between the rows' ends and the
+ * next rows are neither read as values nor written.  Scales are dense:
+ * [n_mats, ceil(n_rows / block_rows), ceil(ne0 / 128)].  Rows, columns and
+ * matrices are below 2^31 each.  Strides count elements (bytes for codes).
+ * Outputs may not overlap inputs. */
+
+/* Encode n_mats matrices of n_rows rows (device pointers); source rows may
+ * start at any element boundary and overlap. */
+int shc_encode_f8(shc_ctx *ctx, uint32_t src_type, const void *src, int64_t n_mats, int64_t n_rows, int64_t ne0,
+                  int64_t row_stride, int64_t mat_stride, int block_rows, uint8_t *codes, int64_t code_row_stride,
+                  int64_t code_mat_stride, float *scales, void *stream);
+
+/* Decode to dense rows of dst_type (SHC_SRC_*): the f32 product code * scale,
+ * rounded once to dst_type. */
+int shc_decode_f8(shc_ctx *ctx, uint32_t dst_type, const uint8_t *codes, int64_t n_mats, int64_t n_rows, int64_t ne0,
+                  int64_t code_row_stride, int64_t code_mat_stride, int block_rows, const float *scales, void *dst,
+                  void *stream);
+
+/* Product of encoded rows with an encoded weight w [n, k] (block_rows 128):
+ *   transposed 0: dst [n_rows, n] = A W^T, A [n_rows, k]
+ *   transposed 1: dst [n_rows, k] = A W,   A [n_rows, n]; with the gradient of
+ *                 A W^T's result as A, the gradient of its rows
+ * A is encoded with block_rows 1; its scales are a_scale_stride apart from
+ * row to row.  Each block's 128 products are summed in f32 and scaled by the
+ * f32 product of the two scales; blocks are summed in order in f32, and the
+ * sum is rounded once to dst_type (SHC_SRC_*). */
+int shc_matmul_f8(shc_ctx *ctx, const uint8_t *a, int64_t a_row_stride, const float *a_scales, int64_t a_scale_stride,
+                  int64_t n_rows, const uint8_t *w, int64_t w_row_stride, const float *w_scales, int64_t n, int64_t k,
+                  int transposed, uint32_t dst_type, void *dst, int64_t dst_row_stride, void *stream);
+
+/* The same with n_experts weights [n_experts, n, k]: rows offsets[e] to
+ * offsets[e + 1] of A and dst belong to expert e.  offsets is a device array
+ * of n_experts + 1 non-decreasing int32 (or, with offsets_64, int64) values,
+ * read when the work runs; an expert may have no rows.  Rows before
+ * offsets[0] and from offsets[n_experts] on are left as they are in dst.
+ * Offsets outside [0, n_rows] are read as the nearest of the two, and an
+ * expert whose offsets decrease has no rows. */
+int shc_matmul_f8_grouped(shc_ctx *ctx, const uint8_t *a, int64_t a_row_stride, const float *a_scales,
+                          int64_t a_scale_stride, int64_t n_rows, const uint8_t *w, int64_t w_row_stride,
+                          int64_t w_mat_stride, const float *w_scales, int64_t n_experts, int64_t n, int64_t k,
+                          const void *offsets, int offsets_64, int transposed, uint32_t dst_type, void *dst,
+                          int64_t dst_row_stride, void *stream);
+
 /* Number of kernel launches issued by this context so far (instrumentation
  * for benchmarks). */
 int64_t shc_launch_count(const shc_ctx *ctx);

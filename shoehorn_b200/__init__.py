@@ -111,6 +111,12 @@ def lib():
         L.shc_row_errors_host.argtypes = [_vp, _vp, _i32, _u32, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i64]
         L.shc_launch_count.restype = _i64
         L.shc_launch_count.argtypes = [_vp]
+        L.shc_encode_f8.argtypes = [_vp, _u32, _vp, _i64, _i64, _i64, _i64, _i64, _i32, _vp, _i64, _i64, _vp, _vp]
+        L.shc_decode_f8.argtypes = [_vp, _u32, _vp, _i64, _i64, _i64, _i64, _i64, _i32, _vp, _vp, _vp]
+        L.shc_matmul_f8.argtypes = [_vp, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _u32, _vp,
+                                    _i64, _vp]
+        L.shc_matmul_f8_grouped.argtypes = [_vp, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64,
+                                            _vp, _i32, _i32, _u32, _vp, _i64, _vp]
         L.shc_grid_info.argtypes = [_i32, ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int32),
                                     ctypes.POINTER(ctypes.c_int64), _vp, _vp]
         _lib = L
@@ -254,6 +260,218 @@ class Context:
         if sync:
             self.sync(stream)
         return err
+
+    # ---------------- 8-bit blocks ----------------
+    # E4M3 codes with one f32 scale for each block of 128 columns (block_rows
+    # 1: activations, gradients) or of 128 x 128 elements (block_rows 128:
+    # weights), value = code * scale; include/shoehorn_cuda.h has the rules.
+    # Every tensor has to be on the context's device.  Work goes to `stream`
+    # (default: torch's current stream of that device); inputs have to be
+    # ready there, and results made here belong to it.
+
+    def _f8_on(self, stream, fresh, *tensors):
+        """Runs `fresh` (the allocation of results) on the stream the work
+        goes to, and keeps the tensors' memory until that work is done where
+        it is not the current one.  Returns (result, stream pointer)."""
+        torch = self.torch
+        if stream is None:
+            return fresh(), self._stream(None)
+        if stream.device.index != self.device:
+            raise ValueError(f"stream of cuda:{stream.device.index} in a context of cuda:{self.device}")
+        if stream == torch.cuda.current_stream(self.device):
+            return fresh(), self._stream(stream)
+        with torch.cuda.stream(stream):
+            made = fresh()
+        for t in tensors:
+            if t is not None:
+                t.record_stream(stream)
+        return made, self._stream(stream)
+
+    def _f8_here(self, t, what):
+        if not t.is_cuda or t.device.index != self.device:
+            raise ValueError(f"{what} must be on cuda:{self.device}")
+
+    def _f8_codes(self, t, what, dims):
+        """(row stride, matrix stride) in bytes of a tensor of codes."""
+        torch = self.torch
+        self._f8_here(t, what)
+        if t.dtype != torch.float8_e4m3fn and t.dtype != torch.uint8:
+            raise TypeError(f"{what} must be float8_e4m3fn (or its bytes as uint8)")
+        if t.dim() not in dims:
+            raise ValueError(f"{what} must have {' or '.join(map(str, dims))} dimensions")
+        rows, cols = t.shape[-2:]
+        if cols < 1:
+            raise ValueError(f"{what} has no columns")
+        if cols > 1 and t.stride(-1) != 1:
+            raise ValueError(f"{what}'s columns must be adjacent")
+        pitch = t.stride(-2) if rows > 1 else -(-cols // 16) * 16
+        mats = t.shape[0] if t.dim() == 3 else 1
+        step = t.stride(0) if mats > 1 else rows * pitch
+        if t.data_ptr() % 16 or pitch % 16 or step % 16:
+            raise ValueError(f"{what}'s rows must start on 16-byte boundaries, as encode_f8 lays them out")
+        if pitch < cols or step < (rows - 1) * pitch + cols:
+            raise ValueError(f"{what}'s rows overlap")
+        return pitch, step
+
+    def _f8_scales(self, t, what, shape):
+        """Row stride of a tensor of scales; only [rows, blocks] may be strided."""
+        self._f8_here(t, what)
+        if t.dtype != self.torch.float32:
+            raise TypeError(f"{what} must be float32")
+        if tuple(t.shape) != shape:
+            raise ValueError(f"{what} must have shape {list(shape)}, not {list(t.shape)}")
+        return t.stride(-2) if shape[-2] > 1 else shape[-1]
+
+    def _f8_dtype(self, dtype):
+        torch = self.torch
+        st = {torch.bfloat16: SRC_BF16, torch.float16: SRC_F16, torch.float32: SRC_F32}.get(dtype)
+        if st is None:
+            raise TypeError(f"unsupported dtype {dtype}")
+        return st
+
+    @staticmethod
+    def _f8_blocks(shape, block_rows):
+        if block_rows not in (1, 128):
+            raise ValueError("block_rows must be 1 or 128")
+        return (*shape[:-2], -(-shape[-2] // block_rows), -(-shape[-1] // 128))
+
+    def encode_f8(self, src, block_rows=1, out=None, scales=None, stream=None, sync=False):
+        """Encode a [rows, cols] or [matrices, rows, cols] CUDA tensor
+        (bf16/f16/f32, adjacent columns, any other strides) to 8-bit blocks.
+
+        Returns (codes, scales): codes float8_e4m3fn of src's shape, each row
+        on a 16-byte boundary; scales float32 [.., ceil(rows / block_rows),
+        ceil(cols / 128)]."""
+        torch = self.torch
+        self._f8_here(src, "src")
+        st = self._f8_dtype(src.dtype)
+        if src.dim() not in (2, 3):
+            raise ValueError("src must have 2 or 3 dimensions")
+        blocks = self._f8_blocks(src.shape, block_rows)
+        rows, cols = src.shape[-2:]
+        mats = src.shape[0] if src.dim() == 3 else 1
+        if cols < 1:
+            raise ValueError("src has no columns")
+        if cols > 1 and src.stride(-1) != 1:
+            raise ValueError("src's columns must be adjacent")
+        if out is not None and tuple(out.shape) != tuple(src.shape):
+            raise ValueError("out must have src's shape")
+        if scales is not None and not scales.is_contiguous():
+            raise ValueError("scales must be contiguous")
+
+        def fresh():
+            o, s = out, scales
+            if o is None:
+                pitch = -(-cols // 16) * 16
+                o = torch.empty((*src.shape[:-1], pitch), dtype=torch.float8_e4m3fn, device=src.device)
+                if pitch != cols:
+                    o = o[..., :cols]
+            if s is None:
+                s = torch.empty(blocks, dtype=torch.float32, device=src.device)
+            return o, s
+
+        (codes, scales), stp = self._f8_on(stream, fresh, src, out, scales)
+        pitch, step = self._f8_codes(codes, "out", (2, 3))
+        self._f8_scales(scales, "scales", blocks)
+        _check(lib().shc_encode_f8(self.handle, st, src.data_ptr(), mats, rows, cols,
+                                   src.stride(-2) if rows > 1 else cols, src.stride(0) if mats > 1 else 0, block_rows,
+                                   codes.data_ptr(), pitch, step, scales.data_ptr(), stp), "encode_f8")
+        if sync:
+            self.sync(stream)
+        return codes, scales
+
+    def decode_f8(self, codes, scales, block_rows=1, dtype=None, out=None, stream=None, sync=False):
+        """The numbers that codes and scales of encode_f8 stand for, as a
+        contiguous tensor of `dtype` (default float32): code * scale, rounded once."""
+        torch = self.torch
+        dtype = dtype or (torch.float32 if out is None else out.dtype)
+        dt = self._f8_dtype(dtype)
+        pitch, step = self._f8_codes(codes, "codes", (2, 3))
+        self._f8_scales(scales, "scales", self._f8_blocks(codes.shape, block_rows))
+        if not scales.is_contiguous():
+            raise ValueError("scales must be contiguous")
+        if out is not None:
+            self._f8_here(out, "out")
+            if out.dtype != dtype or out.shape != codes.shape or not out.is_contiguous():
+                raise ValueError("out must be contiguous, of codes' shape and of dtype")
+
+        def fresh():
+            return torch.empty(codes.shape, dtype=dtype, device=codes.device) if out is None else out
+
+        res, stp = self._f8_on(stream, fresh, codes, scales, out)
+        mats = codes.shape[0] if codes.dim() == 3 else 1
+        _check(lib().shc_decode_f8(self.handle, dt, codes.data_ptr(), mats, codes.shape[-2], codes.shape[-1], pitch,
+                                   step, block_rows, scales.data_ptr(), res.data_ptr(), stp), "decode_f8")
+        if sync:
+            self.sync(stream)
+        return res
+
+    def _f8_product(self, a, a_scales, w, w_scales, offsets, transposed, dtype, out, stream, sync):
+        torch = self.torch
+        n, k = w.shape[-2:]
+        inner, cols = (n, k) if transposed else (k, n)
+        pitch_a, _ = self._f8_codes(a, "a", (2,))
+        pitch_w, step_w = self._f8_codes(w, "w", (2,) if offsets is None else (3,))
+        rows = a.shape[0]
+        if a.shape[1] != inner:
+            raise ValueError(f"a has {a.shape[1]} columns and w {'rows' if transposed else 'columns'} of {inner}")
+        sa = self._f8_scales(a_scales, "a_scales", (rows, -(-inner // 128)))
+        if inner > 128 and a_scales.stride(1) != 1:
+            raise ValueError("a_scales' columns must be adjacent")
+        if sa < a_scales.shape[1]:
+            raise ValueError("a_scales' rows overlap")
+        self._f8_scales(w_scales, "w_scales", self._f8_blocks(w.shape, 128))
+        if not w_scales.is_contiguous():
+            raise ValueError("w_scales must be contiguous")
+        dtype = dtype or (torch.bfloat16 if out is None else out.dtype)
+        dt = self._f8_dtype(dtype)
+        if out is not None:
+            self._f8_here(out, "out")
+            if out.dtype != dtype or tuple(out.shape) != (rows, cols):
+                raise ValueError(f"out must be {dtype} of shape {[rows, cols]}")
+            if (cols > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < cols):
+                raise ValueError("out's columns must be adjacent and its rows apart")
+
+        def fresh():
+            return torch.empty((rows, cols), dtype=dtype, device=a.device) if out is None else out
+
+        res, stp = self._f8_on(stream, fresh, a, a_scales, w, w_scales, offsets, out)
+        pitch_o = res.stride(0) if rows > 1 else cols
+        if offsets is None:
+            _check(lib().shc_matmul_f8(self.handle, a.data_ptr(), pitch_a, a_scales.data_ptr(), sa, rows, w.data_ptr(),
+                                       pitch_w, w_scales.data_ptr(), n, k, transposed, dt, res.data_ptr(), pitch_o, stp),
+                   "matmul_f8")
+        else:
+            _check(lib().shc_matmul_f8_grouped(self.handle, a.data_ptr(), pitch_a, a_scales.data_ptr(), sa, rows,
+                                               w.data_ptr(), pitch_w, step_w, w_scales.data_ptr(), w.shape[0], n, k,
+                                               offsets.data_ptr(), offsets.dtype == torch.int64, transposed, dt,
+                                               res.data_ptr(), pitch_o, stp), "matmul_f8_grouped")
+        if sync:
+            self.sync(stream)
+        return res
+
+    def matmul_f8(self, a, a_scales, w, w_scales, transposed=False, dtype=None, out=None, stream=None, sync=False):
+        """A W^T of encoded rows a [rows, k] (block_rows 1) and an encoded
+        weight w [n, k] (block_rows 128), as [rows, n] of `dtype` (default
+        bfloat16).  transposed: A W with a [rows, n], as [rows, k] (the
+        gradient of the rows, given the encoded gradient of the product).
+        Sums are f32, rounded once."""
+        return self._f8_product(a, a_scales, w, w_scales, None, bool(transposed), dtype, out, stream, sync)
+
+    def matmul_f8_grouped(self, a, a_scales, w, w_scales, offsets, transposed=False, dtype=None, out=None, stream=None,
+                          sync=False):
+        """matmul_f8 with one weight per expert, w [experts, n, k]: rows
+        offsets[e] to offsets[e + 1] of a meet w[e].  offsets: non-decreasing
+        int32 or int64 CUDA tensor [experts + 1], read on the device when the
+        work runs.  Rows of no expert (before offsets[0], from
+        offsets[experts] on) are not written."""
+        torch = self.torch
+        self._f8_here(offsets, "offsets")
+        if offsets.dtype not in (torch.int32, torch.int64):
+            raise TypeError("offsets must be int32 or int64")
+        if w.dim() != 3 or tuple(offsets.shape) != (w.shape[0] + 1,) or not offsets.is_contiguous():
+            raise ValueError("w must be [experts, n, k] and offsets a contiguous [experts + 1]")
+        return self._f8_product(a, a_scales, w, w_scales, offsets, bool(transposed), dtype, out, stream, sync)
 
     # ---------------- host-buffer API ----------------
     def encode_tensor_host(self, ty, src, im=None, rows_per_mat=0, row0=0, out=None, timeout_ms=600_000):

@@ -11,6 +11,7 @@
 #include <thread>
 #include <vector>
 
+#include "f8.cuh"
 #include "iq_host.h"
 #include "kernels.cuh"
 #include "shoehorn_cuda.h"
@@ -266,6 +267,40 @@ bool is_pinned(const void *p) {
         return false;
     }
     return attr.type == cudaMemoryTypeHost;
+}
+
+// A matrix (or n_mats of them) of 8-bit codes: rows on 16-byte boundaries,
+// and sizes that TMA coordinates and strides can hold.
+bool f8_codes_ok(const void *p, int64_t n_mats, int64_t n_rows, int64_t cols, int64_t row_stride, int64_t mat_stride) {
+    constexpr int64_t kMaxDim = INT32_MAX, kMaxStride = (int64_t)1 << 40;
+    if (n_mats > kMaxDim || n_rows > kMaxDim || cols < 1 || cols > kMaxDim) return false;
+    if (((uintptr_t)p & 15) != 0 || row_stride % 16 != 0 || row_stride < cols || row_stride >= kMaxStride) return false;
+    if (n_mats > 1 && (mat_stride % 16 != 0 || mat_stride >= kMaxStride || mat_stride / row_stride < n_rows - 1 ||
+                       mat_stride < (n_rows - 1) * row_stride + cols))
+        return false;
+    return true;
+}
+
+int f8_product(shc_ctx *ctx, F8Product p, void *stream) {
+    if (!ctx || p.n_rows < 0 || p.n_experts < 0 || p.n < 1 || p.k < 1 || !valid_src_type((uint32_t)p.dst_type))
+        return SHC_EINVAL;
+    const int64_t inner = p.transposed ? p.n : p.k, out = p.transposed ? p.k : p.n;
+    if (!f8_codes_ok(p.a, 1, p.n_rows, inner, p.a_row_stride, 0) ||
+        !f8_codes_ok(p.w, p.n_experts, p.n, p.k, p.w_row_stride, p.w_mat_stride))
+        return SHC_EINVAL;
+    if (p.a_scale_stride < (inner + kF8Block - 1) / kF8Block || p.dst_row_stride < out) return SHC_EINVAL;
+    if (((uintptr_t)p.a_scales & 3) || ((uintptr_t)p.w_scales & 3) ||
+        ((uintptr_t)p.dst & (src_elem_bytes((uint32_t)p.dst_type) - 1)) || ((uintptr_t)p.offsets & (p.offsets_64 ? 7 : 3)))
+        return SHC_EINVAL;
+    if (p.n_rows == 0 || p.n_experts == 0) return SHC_OK;
+    if (!p.a || !p.a_scales || !p.w || !p.w_scales || !p.dst) return SHC_EINVAL;
+    if (p.n_experts == 1) p.w_mat_stride = p.n * p.w_row_stride;  // the one matrix may come with any
+    if (p.w_mat_stride >= ((int64_t)1 << 40)) return SHC_EINVAL;
+    DevGuard g(ctx->device);
+    p.status = ctx->d_status;
+    const int rc = launch_f8_product(p, ctx->num_sms, (cudaStream_t)stream);
+    if (rc == SHC_OK) ctx->launches++;
+    return rc;
 }
 
 }  // namespace
@@ -697,6 +732,110 @@ int shc_grid_info(int which, int32_t *grid_size, int32_t *map_size, int64_t *n_n
     if (map_out) std::memcpy(map_out, t.kmap.data(), t.kmap.size() * 4);
     if (neighbours_out) std::memcpy(neighbours_out, t.neighbours.data(), t.neighbours.size() * 4);
     return SHC_OK;
+}
+
+int shc_encode_f8(shc_ctx *ctx, uint32_t src_type, const void *src, int64_t n_mats, int64_t n_rows, int64_t ne0,
+                  int64_t row_stride, int64_t mat_stride, int block_rows, uint8_t *codes, int64_t code_row_stride,
+                  int64_t code_mat_stride, float *scales, void *stream) {
+    if (!ctx || !valid_src_type(src_type) || n_mats < 0 || n_rows < 0 || ne0 < 1) return SHC_EINVAL;
+    if ((block_rows != 1 && block_rows != kF8Block) || row_stride < 0 || mat_stride < 0) return SHC_EINVAL;
+    if (!f8_codes_ok(codes, n_mats, n_rows, ne0, code_row_stride, code_mat_stride)) return SHC_EINVAL;
+    if (((uintptr_t)src & (src_elem_bytes(src_type) - 1)) || ((uintptr_t)scales & 3)) return SHC_EINVAL;
+    if (n_mats == 0 || n_rows == 0) return SHC_OK;
+    if (!src || !codes || !scales) return SHC_EINVAL;
+    DevGuard g(ctx->device);
+    F8Codec c{};
+    c.src = src;
+    c.type = (int)src_type;
+    c.src_row_stride = row_stride;
+    c.src_mat_stride = mat_stride;
+    c.codes = codes;
+    c.code_row_stride = code_row_stride;
+    c.code_mat_stride = code_mat_stride;
+    c.scales = scales;
+    c.n_mats = n_mats;
+    c.n_rows = n_rows;
+    c.ne0 = ne0;
+    c.block_rows = block_rows;
+    const cudaError_t e = launch_f8_encode(c, ctx->num_sms, (cudaStream_t)stream);
+    ctx->launches++;
+    return cuda_status(e);
+}
+
+int shc_decode_f8(shc_ctx *ctx, uint32_t dst_type, const uint8_t *codes, int64_t n_mats, int64_t n_rows, int64_t ne0,
+                  int64_t code_row_stride, int64_t code_mat_stride, int block_rows, const float *scales, void *dst,
+                  void *stream) {
+    if (!ctx || !valid_src_type(dst_type) || n_mats < 0 || n_rows < 0 || ne0 < 1) return SHC_EINVAL;
+    if (block_rows != 1 && block_rows != kF8Block) return SHC_EINVAL;
+    if (!f8_codes_ok(codes, n_mats, n_rows, ne0, code_row_stride, code_mat_stride)) return SHC_EINVAL;
+    if (((uintptr_t)dst & (src_elem_bytes(dst_type) - 1)) || ((uintptr_t)scales & 3)) return SHC_EINVAL;
+    if (n_mats == 0 || n_rows == 0) return SHC_OK;
+    if (!codes || !scales || !dst) return SHC_EINVAL;
+    DevGuard g(ctx->device);
+    F8Codec c{};
+    c.type = (int)dst_type;
+    c.codes = const_cast<uint8_t *>(codes);
+    c.code_row_stride = code_row_stride;
+    c.code_mat_stride = code_mat_stride;
+    c.scales = const_cast<float *>(scales);
+    c.dst = dst;
+    c.n_mats = n_mats;
+    c.n_rows = n_rows;
+    c.ne0 = ne0;
+    c.block_rows = block_rows;
+    const cudaError_t e = launch_f8_decode(c, ctx->num_sms, (cudaStream_t)stream);
+    ctx->launches++;
+    return cuda_status(e);
+}
+
+int shc_matmul_f8(shc_ctx *ctx, const uint8_t *a, int64_t a_row_stride, const float *a_scales, int64_t a_scale_stride,
+                  int64_t n_rows, const uint8_t *w, int64_t w_row_stride, const float *w_scales, int64_t n, int64_t k,
+                  int transposed, uint32_t dst_type, void *dst, int64_t dst_row_stride, void *stream) {
+    F8Product p{};
+    p.a = a;
+    p.a_scales = a_scales;
+    p.a_row_stride = a_row_stride;
+    p.a_scale_stride = a_scale_stride;
+    p.n_rows = n_rows;
+    p.w = w;
+    p.w_scales = w_scales;
+    p.w_row_stride = w_row_stride;
+    p.n_experts = 1;
+    p.n = n;
+    p.k = k;
+    p.transposed = transposed != 0;
+    p.dst_type = (int)dst_type;
+    p.dst = dst;
+    p.dst_row_stride = dst_row_stride;
+    return f8_product(ctx, p, stream);
+}
+
+int shc_matmul_f8_grouped(shc_ctx *ctx, const uint8_t *a, int64_t a_row_stride, const float *a_scales,
+                          int64_t a_scale_stride, int64_t n_rows, const uint8_t *w, int64_t w_row_stride,
+                          int64_t w_mat_stride, const float *w_scales, int64_t n_experts, int64_t n, int64_t k,
+                          const void *offsets, int offsets_64, int transposed, uint32_t dst_type, void *dst,
+                          int64_t dst_row_stride, void *stream) {
+    if (!offsets) return SHC_EINVAL;
+    F8Product p{};
+    p.a = a;
+    p.a_scales = a_scales;
+    p.a_row_stride = a_row_stride;
+    p.a_scale_stride = a_scale_stride;
+    p.n_rows = n_rows;
+    p.w = w;
+    p.w_scales = w_scales;
+    p.w_row_stride = w_row_stride;
+    p.w_mat_stride = w_mat_stride;
+    p.n_experts = n_experts;
+    p.n = n;
+    p.k = k;
+    p.offsets = offsets;
+    p.offsets_64 = offsets_64 != 0;
+    p.transposed = transposed != 0;
+    p.dst_type = (int)dst_type;
+    p.dst = dst;
+    p.dst_row_stride = dst_row_stride;
+    return f8_product(ctx, p, stream);
 }
 
 }  // extern "C"
