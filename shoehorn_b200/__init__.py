@@ -90,6 +90,8 @@ _vp, _i64, _u32, _i32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_uint32, ctypes
 def lib():
     """Load libshoehorn_cuda.so (raises if it was not built)."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lib_lock:
         if _lib is not None:
             return _lib
@@ -268,72 +270,93 @@ class Context:
     # Every tensor has to be on the context's device.  Work goes to `stream`
     # (default: torch's current stream of that device); inputs have to be
     # ready there, and results made here belong to it.
+    # Single-token calls are bound by the host, so each tensor's size, strides
+    # and device are asked for once.
 
     def _f8_on(self, stream, fresh, *tensors):
-        """Runs `fresh` (the allocation of results) on the stream the work
-        goes to, and keeps the tensors' memory until that work is done where
-        it is not the current one.  Returns (result, stream pointer)."""
+        """Allocates results (`fresh`) on the stream the work goes to, and
+        keeps the tensors' memory until that work is done where it is not the
+        current one.  Returns (results, stream handle)."""
         torch = self.torch
         if stream is None:
-            return fresh(), self._stream(None)
+            return fresh(), self._f8_stream()
         if stream.device.index != self.device:
             raise ValueError(f"stream of cuda:{stream.device.index} in a context of cuda:{self.device}")
         if stream == torch.cuda.current_stream(self.device):
-            return fresh(), self._stream(stream)
+            return fresh(), stream.cuda_stream
         with torch.cuda.stream(stream):
             made = fresh()
         for t in tensors:
             if t is not None:
                 t.record_stream(stream)
-        return made, self._stream(stream)
+        return made, stream.cuda_stream
+
+    def _f8_stream(self):
+        raw = getattr(self.torch._C, "_cuda_getCurrentRawStream", None)
+        return raw(self.device) if raw else self.torch.cuda.current_stream(self.device).cuda_stream
 
     def _f8_here(self, t, what):
-        if not t.is_cuda or t.device.index != self.device:
+        if t.get_device() != self.device:
             raise ValueError(f"{what} must be on cuda:{self.device}")
 
     def _f8_codes(self, t, what, dims):
-        """(row stride, matrix stride) in bytes of a tensor of codes."""
-        torch = self.torch
+        """(matrices, rows, columns, row stride, matrix stride) of codes; strides in bytes."""
         self._f8_here(t, what)
-        if t.dtype != torch.float8_e4m3fn and t.dtype != torch.uint8:
+        torch = self.torch
+        d = t.dtype
+        if d is not torch.float8_e4m3fn and d is not torch.uint8:
             raise TypeError(f"{what} must be float8_e4m3fn (or its bytes as uint8)")
-        if t.dim() not in dims:
+        shape, stride = t.shape, t.stride()
+        if len(shape) not in dims:
             raise ValueError(f"{what} must have {' or '.join(map(str, dims))} dimensions")
-        rows, cols = t.shape[-2:]
+        if len(shape) == 2:
+            rows, cols = shape
+            mats, step = 1, 0
+            pitch, one = stride
+        else:
+            mats, rows, cols = shape
+            step, pitch, one = stride
+        if one != 1 and cols > 1:
+            raise ValueError(f"{what}'s columns must be adjacent")
+        if rows <= 1:  # a lone row may come with any stride
+            pitch = (cols + 15) // 16 * 16
+        if mats <= 1:
+            step = rows * pitch
         if cols < 1:
             raise ValueError(f"{what} has no columns")
-        if cols > 1 and t.stride(-1) != 1:
-            raise ValueError(f"{what}'s columns must be adjacent")
-        pitch = t.stride(-2) if rows > 1 else -(-cols // 16) * 16
-        mats = t.shape[0] if t.dim() == 3 else 1
-        step = t.stride(0) if mats > 1 else rows * pitch
         if t.data_ptr() % 16 or pitch % 16 or step % 16:
             raise ValueError(f"{what}'s rows must start on 16-byte boundaries, as encode_f8 lays them out")
         if pitch < cols or step < (rows - 1) * pitch + cols:
             raise ValueError(f"{what}'s rows overlap")
-        return pitch, step
+        return mats, rows, cols, pitch, step
 
-    def _f8_scales(self, t, what, shape):
-        """Row stride of a tensor of scales; only [rows, blocks] may be strided."""
+    def _f8_scales(self, t, what, shape, strided=False):
+        """Row stride of scales of the given shape; contiguous unless strided."""
         self._f8_here(t, what)
-        if t.dtype != self.torch.float32:
+        if t.dtype is not self.torch.float32:
             raise TypeError(f"{what} must be float32")
-        if tuple(t.shape) != shape:
+        if t.shape != shape:
             raise ValueError(f"{what} must have shape {list(shape)}, not {list(t.shape)}")
-        return t.stride(-2) if shape[-2] > 1 else shape[-1]
+        if t.is_contiguous():
+            return shape[-1]
+        if not strided:
+            raise ValueError(f"{what} must be contiguous")
+        pitch, one = t.stride()
+        if shape[0] <= 1:
+            pitch = shape[1]
+        if (one != 1 and shape[1] > 1) or pitch < shape[1]:
+            raise ValueError(f"{what}'s columns must be adjacent and its rows apart")
+        return pitch
 
     def _f8_dtype(self, dtype):
         torch = self.torch
-        st = {torch.bfloat16: SRC_BF16, torch.float16: SRC_F16, torch.float32: SRC_F32}.get(dtype)
-        if st is None:
-            raise TypeError(f"unsupported dtype {dtype}")
-        return st
-
-    @staticmethod
-    def _f8_blocks(shape, block_rows):
-        if block_rows not in (1, 128):
-            raise ValueError("block_rows must be 1 or 128")
-        return (*shape[:-2], -(-shape[-2] // block_rows), -(-shape[-1] // 128))
+        if dtype is torch.bfloat16:
+            return SRC_BF16
+        if dtype is torch.float32:
+            return SRC_F32
+        if dtype is torch.float16:
+            return SRC_F16
+        raise TypeError(f"unsupported dtype {dtype}")
 
     def encode_f8(self, src, block_rows=1, out=None, scales=None, stream=None, sync=False):
         """Encode a [rows, cols] or [matrices, rows, cols] CUDA tensor
@@ -345,40 +368,47 @@ class Context:
         torch = self.torch
         self._f8_here(src, "src")
         st = self._f8_dtype(src.dtype)
-        if src.dim() not in (2, 3):
+        shape, stride = src.shape, src.stride()
+        if len(shape) not in (2, 3):
             raise ValueError("src must have 2 or 3 dimensions")
-        blocks = self._f8_blocks(src.shape, block_rows)
-        rows, cols = src.shape[-2:]
-        mats = src.shape[0] if src.dim() == 3 else 1
+        if block_rows != 1 and block_rows != 128:
+            raise ValueError("block_rows must be 1 or 128")
+        rows, cols = shape[-2:]
+        lead = tuple(shape[:-2])
+        mats = lead[0] if lead else 1
         if cols < 1:
             raise ValueError("src has no columns")
-        if cols > 1 and src.stride(-1) != 1:
+        if cols > 1 and stride[-1] != 1:
             raise ValueError("src's columns must be adjacent")
-        if out is not None and tuple(out.shape) != tuple(src.shape):
+        if out is not None and out.shape != shape:
             raise ValueError("out must have src's shape")
-        if scales is not None and not scales.is_contiguous():
-            raise ValueError("scales must be contiguous")
+        blocks = (*lead, -(-rows // block_rows), (cols + 127) // 128)
+        pitch = (cols + 15) // 16 * 16
+        step = rows * pitch
 
         def fresh():
             o, s = out, scales
             if o is None:
-                pitch = -(-cols // 16) * 16
-                o = torch.empty((*src.shape[:-1], pitch), dtype=torch.float8_e4m3fn, device=src.device)
+                o = torch.empty((*lead, rows, pitch), dtype=torch.float8_e4m3fn, device=src.device)
                 if pitch != cols:
                     o = o[..., :cols]
             if s is None:
                 s = torch.empty(blocks, dtype=torch.float32, device=src.device)
             return o, s
 
-        (codes, scales), stp = self._f8_on(stream, fresh, src, out, scales)
-        pitch, step = self._f8_codes(codes, "out", (2, 3))
-        self._f8_scales(scales, "scales", blocks)
-        _check(lib().shc_encode_f8(self.handle, st, src.data_ptr(), mats, rows, cols,
-                                   src.stride(-2) if rows > 1 else cols, src.stride(0) if mats > 1 else 0, block_rows,
-                                   codes.data_ptr(), pitch, step, scales.data_ptr(), stp), "encode_f8")
+        (codes, made), stp = self._f8_on(stream, fresh, src, out, scales)
+        if out is not None:
+            pitch, step = self._f8_codes(out, "out", (2, 3))[3:]
+        if scales is not None:
+            self._f8_scales(scales, "scales", blocks)
+        rc = lib().shc_encode_f8(self.handle, st, src.data_ptr(), mats, rows, cols, stride[-2] if rows > 1 else cols,
+                                 stride[0] if mats > 1 else 0, block_rows, codes.data_ptr(), pitch, step,
+                                 made.data_ptr(), stp)
+        if rc:
+            raise ShoehornError(rc, "encode_f8")
         if sync:
             self.sync(stream)
-        return codes, scales
+        return codes, made
 
     def decode_f8(self, codes, scales, block_rows=1, dtype=None, out=None, stream=None, sync=False):
         """The numbers that codes and scales of encode_f8 stand for, as a
@@ -386,66 +416,65 @@ class Context:
         torch = self.torch
         dtype = dtype or (torch.float32 if out is None else out.dtype)
         dt = self._f8_dtype(dtype)
-        pitch, step = self._f8_codes(codes, "codes", (2, 3))
-        self._f8_scales(scales, "scales", self._f8_blocks(codes.shape, block_rows))
-        if not scales.is_contiguous():
-            raise ValueError("scales must be contiguous")
+        if block_rows != 1 and block_rows != 128:
+            raise ValueError("block_rows must be 1 or 128")
+        mats, rows, cols, pitch, step = self._f8_codes(codes, "codes", (2, 3))
+        shape = codes.shape
+        self._f8_scales(scales, "scales", (*shape[:-2], -(-rows // block_rows), (cols + 127) // 128))
         if out is not None:
             self._f8_here(out, "out")
-            if out.dtype != dtype or out.shape != codes.shape or not out.is_contiguous():
+            if out.dtype is not dtype or out.shape != shape or not out.is_contiguous():
                 raise ValueError("out must be contiguous, of codes' shape and of dtype")
 
         def fresh():
-            return torch.empty(codes.shape, dtype=dtype, device=codes.device) if out is None else out
+            return torch.empty(shape, dtype=dtype, device=codes.device) if out is None else out
 
         res, stp = self._f8_on(stream, fresh, codes, scales, out)
-        mats = codes.shape[0] if codes.dim() == 3 else 1
-        _check(lib().shc_decode_f8(self.handle, dt, codes.data_ptr(), mats, codes.shape[-2], codes.shape[-1], pitch,
-                                   step, block_rows, scales.data_ptr(), res.data_ptr(), stp), "decode_f8")
+        rc = lib().shc_decode_f8(self.handle, dt, codes.data_ptr(), mats, rows, cols, pitch, step, block_rows,
+                                 scales.data_ptr(), res.data_ptr(), stp)
+        if rc:
+            raise ShoehornError(rc, "decode_f8")
         if sync:
             self.sync(stream)
         return res
 
     def _f8_product(self, a, a_scales, w, w_scales, offsets, transposed, dtype, out, stream, sync):
         torch = self.torch
-        n, k = w.shape[-2:]
+        _, rows, a_cols, pitch_a, _ = self._f8_codes(a, "a", (2,))
+        experts, n, k, pitch_w, step_w = self._f8_codes(w, "w", (2,) if offsets is None else (3,))
         inner, cols = (n, k) if transposed else (k, n)
-        pitch_a, _ = self._f8_codes(a, "a", (2,))
-        pitch_w, step_w = self._f8_codes(w, "w", (2,) if offsets is None else (3,))
-        rows = a.shape[0]
-        if a.shape[1] != inner:
-            raise ValueError(f"a has {a.shape[1]} columns and w {'rows' if transposed else 'columns'} of {inner}")
-        sa = self._f8_scales(a_scales, "a_scales", (rows, -(-inner // 128)))
-        if inner > 128 and a_scales.stride(1) != 1:
-            raise ValueError("a_scales' columns must be adjacent")
-        if sa < a_scales.shape[1]:
-            raise ValueError("a_scales' rows overlap")
-        self._f8_scales(w_scales, "w_scales", self._f8_blocks(w.shape, 128))
-        if not w_scales.is_contiguous():
-            raise ValueError("w_scales must be contiguous")
-        dtype = dtype or (torch.bfloat16 if out is None else out.dtype)
+        if a_cols != inner:
+            raise ValueError(f"a has {a_cols} columns and w {inner} {'rows' if transposed else 'columns'}")
+        pitch_s = self._f8_scales(a_scales, "a_scales", (rows, (inner + 127) // 128), strided=True)
+        blocks = ((n + 127) // 128, (k + 127) // 128)
+        self._f8_scales(w_scales, "w_scales", blocks if offsets is None else (experts, *blocks))
+        if dtype is None:
+            dtype = torch.bfloat16 if out is None else out.dtype
         dt = self._f8_dtype(dtype)
+        pitch_o = cols
         if out is not None:
             self._f8_here(out, "out")
-            if out.dtype != dtype or tuple(out.shape) != (rows, cols):
+            if out.dtype is not dtype or out.shape != (rows, cols):
                 raise ValueError(f"out must be {dtype} of shape {[rows, cols]}")
-            if (cols > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < cols):
+            if rows > 1:
+                pitch_o = out.stride(0)
+            if (cols > 1 and out.stride(1) != 1) or pitch_o < cols:
                 raise ValueError("out's columns must be adjacent and its rows apart")
 
         def fresh():
             return torch.empty((rows, cols), dtype=dtype, device=a.device) if out is None else out
 
         res, stp = self._f8_on(stream, fresh, a, a_scales, w, w_scales, offsets, out)
-        pitch_o = res.stride(0) if rows > 1 else cols
         if offsets is None:
-            _check(lib().shc_matmul_f8(self.handle, a.data_ptr(), pitch_a, a_scales.data_ptr(), sa, rows, w.data_ptr(),
-                                       pitch_w, w_scales.data_ptr(), n, k, transposed, dt, res.data_ptr(), pitch_o, stp),
-                   "matmul_f8")
+            rc = lib().shc_matmul_f8(self.handle, a.data_ptr(), pitch_a, a_scales.data_ptr(), pitch_s, rows, w.data_ptr(),
+                                     pitch_w, w_scales.data_ptr(), n, k, transposed, dt, res.data_ptr(), pitch_o, stp)
         else:
-            _check(lib().shc_matmul_f8_grouped(self.handle, a.data_ptr(), pitch_a, a_scales.data_ptr(), sa, rows,
-                                               w.data_ptr(), pitch_w, step_w, w_scales.data_ptr(), w.shape[0], n, k,
-                                               offsets.data_ptr(), offsets.dtype == torch.int64, transposed, dt,
-                                               res.data_ptr(), pitch_o, stp), "matmul_f8_grouped")
+            rc = lib().shc_matmul_f8_grouped(self.handle, a.data_ptr(), pitch_a, a_scales.data_ptr(), pitch_s, rows,
+                                             w.data_ptr(), pitch_w, step_w, w_scales.data_ptr(), experts, n, k,
+                                             offsets.data_ptr(), offsets.dtype is torch.int64, transposed, dt,
+                                             res.data_ptr(), pitch_o, stp)
+        if rc:
+            raise ShoehornError(rc, "matmul_f8" if offsets is None else "matmul_f8_grouped")
         if sync:
             self.sync(stream)
         return res
@@ -467,9 +496,9 @@ class Context:
         offsets[experts] on) are not written."""
         torch = self.torch
         self._f8_here(offsets, "offsets")
-        if offsets.dtype not in (torch.int32, torch.int64):
+        if offsets.dtype is not torch.int32 and offsets.dtype is not torch.int64:
             raise TypeError("offsets must be int32 or int64")
-        if w.dim() != 3 or tuple(offsets.shape) != (w.shape[0] + 1,) or not offsets.is_contiguous():
+        if w.dim() != 3 or offsets.shape != (w.shape[0] + 1,) or not offsets.is_contiguous():
             raise ValueError("w must be [experts, n, k] and offsets a contiguous [experts + 1]")
         return self._f8_product(a, a_scales, w, w_scales, offsets, bool(transposed), dtype, out, stream, sync)
 

@@ -757,7 +757,7 @@ int shc_encode_f8(shc_ctx *ctx, uint32_t src_type, const void *src, int64_t n_ma
     c.n_rows = n_rows;
     c.ne0 = ne0;
     c.block_rows = block_rows;
-    const cudaError_t e = launch_f8_encode(c, ctx->num_sms, (cudaStream_t)stream);
+    const cudaError_t e = launch_f8_encode(c, (cudaStream_t)stream);
     ctx->launches++;
     return cuda_status(e);
 }
@@ -783,7 +783,7 @@ int shc_decode_f8(shc_ctx *ctx, uint32_t dst_type, const uint8_t *codes, int64_t
     c.n_rows = n_rows;
     c.ne0 = ne0;
     c.block_rows = block_rows;
-    const cudaError_t e = launch_f8_decode(c, ctx->num_sms, (cudaStream_t)stream);
+    const cudaError_t e = launch_f8_decode(c, (cudaStream_t)stream);
     ctx->launches++;
     return cuda_status(e);
 }

@@ -14,11 +14,12 @@
 namespace shc {
 namespace {
 
-constexpr int kLanes = 16;  // lanes of one 128-column block, 8 columns each
+constexpr int kLanes = 8;   // lanes of one 128-column block
+constexpr int kElems = 16;  // columns of one lane: one 16-byte store of codes
 
 // Two E4M3 codes, lo in the low byte; NaN gives 0x7F, magnitudes above 448
 // give 448 (reached only by the rounding of x * (448 / top)).
-__device__ __forceinline__ uint16_t e4m3x2(float lo, float hi) {
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     uint16_t r;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
     return r;
@@ -31,136 +32,200 @@ __device__ __forceinline__ float2 e4m3x2_val(uint16_t c) {
 
 __device__ __forceinline__ float inf_f() { return __uint_as_float(0x7f800000u); }
 
-// Eight columns of a row from `col`, columns at or past ne0 as zeros.
-template <bool VEC>
-__device__ __forceinline__ void load_cols(const RowSrc &s, int64_t row, int64_t col, float v[8]) {
-    if (VEC && col + 8 <= s.ne0) {
-        load8(s, row, col, v);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = col + i < s.ne0 ? load1(s, row, col + i) : 0.0f;
-    }
-}
+// A lane's 16 source elements as they lie in memory.  16-bit types stay
+// packed: half the registers, and the magnitudes' maximum takes two elements
+// per instruction.
+template <int ST>
+struct Raw {
+    static constexpr int kWords = ST == SHC_SRC_F32 ? 16 : 8;
+    uint32_t w[kWords];
 
-// Largest magnitude, NaN ignored; infinite if any element is.
-__device__ __forceinline__ float top8(const float v[8]) {
-    float m = 0.0f;
+    // Columns col.. of the row at p, zeros from ne0 on.
+    template <bool VEC>
+    __device__ __forceinline__ void load(const uint8_t *p, int64_t col, int64_t ne0) {
+        constexpr int esz = ST == SHC_SRC_F32 ? 4 : 2;
+        if (VEC && col + kElems <= ne0) {
+            const uint4 *q = reinterpret_cast<const uint4 *>(p + col * esz);
 #pragma unroll
-    for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(v[i]));
-    return m;
-}
-// Infinite elements to NaN (the NaN code); returns the finite ones' maximum.
-__device__ __forceinline__ float drop_inf8(float v[8]) {
-    float m = 0.0f;
+            for (int i = 0; i < kWords / 4; i++) {
+                const uint4 v = __ldcs(q + i);  // read once
+                w[4 * i] = v.x;
+                w[4 * i + 1] = v.y;
+                w[4 * i + 2] = v.z;
+                w[4 * i + 3] = v.w;
+            }
+        } else if (ST == SHC_SRC_F32) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        if (fabsf(v[i]) == inf_f()) v[i] = __uint_as_float(0x7fffffffu);
-        else m = fmaxf(m, fabsf(v[i]));
-    }
-    return m;
-}
-
-// Codes of eight columns; a whole group is one 8-byte store (codes rows start
-// on 16-byte boundaries), the row's ragged end single bytes.
-__device__ __forceinline__ void store_codes(uint8_t *row, int64_t col, int64_t ne0, const float v[8], float inv) {
-    if (col >= ne0) return;
-    uint32_t w[2];
+            for (int i = 0; i < kWords; i++)
+                w[i] = col + i < ne0 ? __ldg(reinterpret_cast<const uint32_t *>(p) + col + i) : 0u;
+        } else {
+            const uint16_t *q = reinterpret_cast<const uint16_t *>(p) + col;
 #pragma unroll
-    for (int i = 0; i < 2; i++)
-        w[i] = (uint32_t)e4m3x2(v[4 * i] * inv, v[4 * i + 1] * inv) |
-               ((uint32_t)e4m3x2(v[4 * i + 2] * inv, v[4 * i + 3] * inv) << 16);
-    if (col + 8 <= ne0) {
-        *reinterpret_cast<uint2 *>(row + col) = make_uint2(w[0], w[1]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (col + i < ne0) row[col + i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
-    }
-}
-
-// One 16-lane half-warp per (row, block).
-template <bool VEC>
-__global__ void __launch_bounds__(256) f8_encode_rows_kernel(F8Codec c) {
-    const int64_t nb = (c.ne0 + kF8Block - 1) / kF8Block, total = c.n_mats * c.n_rows * nb;
-    const int lane = threadIdx.x & (kLanes - 1);
-    const int64_t step = (int64_t)gridDim.x * (256 / kLanes);
-    const int64_t rounds = (total + step - 1) / step;  // whole warps stay together for the shuffles
-    int64_t u = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
-    for (int64_t i = 0; i < rounds; i++, u += step) {
-        const bool on = u < total;
-        const int64_t row = on ? u / nb : 0, b = on ? u - row * nb : 0;
-        const int64_t mat = row / c.n_rows, r = row - mat * c.n_rows;
-        const int64_t col = b * kF8Block + lane * 8;
-        const size_t esz = c.type == SHC_SRC_F32 ? 4 : 2;
-        const RowSrc s{static_cast<const uint8_t *>(c.src) + mat * c.src_mat_stride * (int64_t)esz, c.type,
-                       on ? c.ne0 : 0, c.src_row_stride};
-        float v[8];
-        load_cols<VEC>(s, r, col, v);
-        float m = top8(v);
-#pragma unroll
-        for (int o = kLanes / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-        if (__any_sync(~0u, m == inf_f())) {
-            m = drop_inf8(v);
-#pragma unroll
-            for (int o = kLanes / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+            for (int i = 0; i < kWords; i++) {
+                const uint32_t lo = col + 2 * i < ne0 ? __ldg(q + 2 * i) : 0u;
+                const uint32_t hi = col + 2 * i + 1 < ne0 ? __ldg(q + 2 * i + 1) : 0u;
+                w[i] = lo | hi << 16;
+            }
         }
-        m = fmaxf(m, kF8Least);
-        if (!on) continue;
-        store_codes(c.codes + mat * c.code_mat_stride + r * c.code_row_stride, col, c.ne0, v, kF8Top / m);
-        if (lane == 0) c.scales[u] = m / kF8Top;
     }
-}
-
-// One thread block per 128 x 128 tile, held in registers between the maximum
-// and the codes: thread t has columns 8 (t % 16).. of rows t / 16 + 16 i.
-template <bool VEC>
-__global__ void __launch_bounds__(256) f8_encode_tiles_kernel(F8Codec c) {
-    const int64_t nb = (c.ne0 + kF8Block - 1) / kF8Block, rb = (c.n_rows + kF8Block - 1) / kF8Block;
-    const int lane = threadIdx.x & (kLanes - 1), r16 = threadIdx.x / kLanes;
-    __shared__ float s_top[2][8];
-    int turn = 0;
-    for (int64_t tile = blockIdx.x; tile < c.n_mats * rb * nb; tile += gridDim.x) {
-        const int64_t b = tile % nb, rest = tile / nb, mat = rest / rb, row0 = (rest - mat * rb) * kF8Block;
-        const int64_t col = b * kF8Block + lane * 8;
-        const size_t esz = c.type == SHC_SRC_F32 ? 4 : 2;
-        const RowSrc s{static_cast<const uint8_t *>(c.src) + mat * c.src_mat_stride * (int64_t)esz, c.type, c.ne0,
-                       c.src_row_stride};
-        float v[8][8];
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < kWords; i++) w[i] = 0;
+    }
+    __device__ __forceinline__ float at(int i) const {
+        if (ST == SHC_SRC_F32) return __uint_as_float(w[i % kWords]);
+        const uint32_t v = w[(i >> 1) % kWords];
+        if (ST == SHC_SRC_BF16) return __uint_as_float(i & 1 ? v & 0xFFFF0000u : v << 16);
+        return f16_val((uint16_t)(i & 1 ? v >> 16 : v));
+    }
+    // Largest magnitude, NaN ignored; infinite if any element is.
+    __device__ __forceinline__ float top() const {
+        if (ST == SHC_SRC_F32) {
+            float m = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kWords; i++) m = fmaxf(m, fabsf(__uint_as_float(w[i])));
+            return m;
+        }
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < kWords; i++) {
+            const uint32_t v = w[i] & 0x7FFF7FFFu;
+            if (ST == SHC_SRC_BF16) asm("max.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(v));
+            else asm("max.f16x2 %0, %0, %1;" : "+r"(m) : "r"(v));
+        }
+        if (ST == SHC_SRC_BF16) return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xFFFF0000u));
+        return fmaxf(f16_val((uint16_t)m), f16_val((uint16_t)(m >> 16)));
+    }
+    // Infinite elements to NaN (the NaN code); returns the finite ones' maximum.
+    __device__ __forceinline__ float drop_inf() {
         float m = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int64_t r = row0 + r16 + 16 * i;
-            if (r < c.n_rows) {
-                load_cols<VEC>(s, r, col, v[i]);
+        for (int i = 0; i < kElems; i++) {
+            const float x = fabsf(at(i));
+            if (x != inf_f()) {
+                m = fmaxf(m, x);
+            } else if (ST == SHC_SRC_F32) {
+                w[i % kWords] = 0x7FFFFFFFu;
             } else {
-#pragma unroll
-                for (int j = 0; j < 8; j++) v[i][j] = 0.0f;
+                w[(i >> 1) % kWords] |= i & 1 ? 0x7FFF0000u : 0x00007FFFu;
             }
-            m = fmaxf(m, top8(v[i]));
         }
-        // Block-wide maximum; the second pass only where an element is infinite.
-        for (int pass = 0; pass < 2; pass++) {
-            for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-            if ((threadIdx.x & 31) == 0) s_top[turn][threadIdx.x / 32] = m;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < 8; w++) m = fmaxf(m, s_top[turn][w]);
-            turn ^= 1;  // the next maximum does not overwrite one still being read
-            if (m != inf_f()) break;
-            m = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; i++) m = fmaxf(m, drop_inf8(v[i]));
-        }
-        m = fmaxf(m, kF8Least);
-        const float inv = kF8Top / m;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int64_t r = row0 + r16 + 16 * i;
-            if (r < c.n_rows)
-                store_codes(c.codes + mat * c.code_mat_stride + r * c.code_row_stride, col, c.ne0, v[i], inv);
-        }
-        if (threadIdx.x == 0) c.scales[tile] = m / kF8Top;
+        return m;
     }
+    // Codes to a row that starts on a 16-byte boundary: one 16-byte store,
+    // the row's ragged end in single bytes.
+    __device__ __forceinline__ void store(uint8_t *row, int64_t col, int64_t ne0, float inv) const {
+        uint32_t q[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            q[i] = e4m3x2(at(4 * i) * inv, at(4 * i + 1) * inv) | e4m3x2(at(4 * i + 2) * inv, at(4 * i + 3) * inv) << 16;
+        if (col + kElems <= ne0) {
+            *reinterpret_cast<uint4 *>(row + col) = make_uint4(q[0], q[1], q[2], q[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kElems; i++)
+                if (col + i < ne0) row[col + i] = (uint8_t)(q[i >> 2] >> (8 * (i & 3)));
+        }
+    }
+};
+
+template <int ST>
+__device__ __forceinline__ const uint8_t *src_row(const F8Codec &c, int64_t mat, int64_t r) {
+    return static_cast<const uint8_t *>(c.src) + (mat * c.src_mat_stride + r * c.src_row_stride) * (ST == SHC_SRC_F32 ? 4 : 2);
+}
+
+// Activations: eight lanes per (row, block), kUnits of them at once so that a
+// warp has kUnits x 4 blocks' loads in flight.  I: unit index type, 32 bits
+// wherever the units can be counted in them (a division by the row's blocks
+// per unit).
+template <int ST>
+__host__ __device__ constexpr int units() { return ST == SHC_SRC_F32 ? 2 : 4; }
+
+template <int ST, bool VEC, typename I>
+__global__ void __launch_bounds__(256) f8_encode_rows_kernel(F8Codec c) {
+    constexpr int kUnits = units<ST>(), kPerBlock = 256 / kLanes;
+    const I nb = (I)((c.ne0 + kF8Block - 1) / kF8Block), total = (I)(c.n_mats * c.n_rows) * nb, rows = (I)c.n_rows;
+    const int lane = threadIdx.x & (kLanes - 1);
+    const I u0 = (I)blockIdx.x * (kPerBlock * kUnits) + threadIdx.x / kLanes;
+    Raw<ST> v[kUnits];
+    uint8_t *row[kUnits];
+    int64_t col[kUnits];
+    float m[kUnits];
+#pragma unroll
+    for (int k = 0; k < kUnits; k++) {
+        const I u = u0 + (I)(k * kPerBlock);
+        const I g = u < total ? u / nb : 0, b = u < total ? u - g * nb : 0;
+        const I mat = c.n_mats > 1 ? g / rows : 0, r = g - mat * rows;
+        col[k] = (int64_t)b * kF8Block + lane * kElems;
+        if (u >= total) col[k] = c.ne0;
+        row[k] = c.codes + (int64_t)mat * c.code_mat_stride + (int64_t)r * c.code_row_stride;
+        v[k].template load<VEC>(src_row<ST>(c, mat, r), col[k], c.ne0);
+    }
+    bool inf = false;
+#pragma unroll
+    for (int k = 0; k < kUnits; k++) {
+        m[k] = v[k].top();
+#pragma unroll
+        for (int o = kLanes / 2; o; o >>= 1) m[k] = fmaxf(m[k], __shfl_xor_sync(~0u, m[k], o));
+        inf |= m[k] == inf_f();
+    }
+    if (__any_sync(~0u, inf)) {
+#pragma unroll
+        for (int k = 0; k < kUnits; k++) {
+            m[k] = v[k].drop_inf();
+#pragma unroll
+            for (int o = kLanes / 2; o; o >>= 1) m[k] = fmaxf(m[k], __shfl_xor_sync(~0u, m[k], o));
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kUnits; k++) {
+        const I u = u0 + (I)(k * kPerBlock);
+        const float t = fmaxf(m[k], kF8Least);
+        if (col[k] < c.ne0) v[k].store(row[k], col[k], c.ne0, kF8Top / t);
+        if (u < total && lane == 0) c.scales[u] = t / kF8Top;
+    }
+}
+
+// Weights: one thread block per 128 x 128 tile, held in registers between the
+// maximum and the codes; thread t has 16 columns of rows t / 8 + 32 i.
+template <int ST, bool VEC>
+__global__ void __launch_bounds__(256) f8_encode_tiles_kernel(F8Codec c) {
+    const int64_t nb = (c.ne0 + kF8Block - 1) / kF8Block, rb = (c.n_rows + kF8Block - 1) / kF8Block;
+    const int64_t tile = blockIdx.x, b = tile % nb, rest = tile / nb, mat = rest / rb;
+    const int64_t row0 = (rest - mat * rb) * kF8Block + threadIdx.x / kLanes;
+    const int64_t col = b * kF8Block + (threadIdx.x & (kLanes - 1)) * kElems;
+    __shared__ float s_top[2][8];
+    Raw<ST> v[4];
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int64_t r = row0 + 32 * i;
+        if (r < c.n_rows) v[i].template load<VEC>(src_row<ST>(c, mat, r), col, c.ne0);
+        else v[i].zero();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) m = fmaxf(m, v[i].top());
+    // Block-wide maximum; a second pass only where an element is infinite.
+    for (int pass = 0; pass < 2; pass++) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+        if ((threadIdx.x & 31) == 0) s_top[pass][threadIdx.x / 32] = m;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 8; w++) m = fmaxf(m, s_top[pass][w]);
+        if (m != inf_f()) break;
+        m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) m = fmaxf(m, v[i].drop_inf());
+    }
+    m = fmaxf(m, kF8Least);
+    const float inv = kF8Top / m;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int64_t r = row0 + 32 * i;
+        if (r < c.n_rows) v[i].store(c.codes + mat * c.code_mat_stride + r * c.code_row_stride, col, c.ne0, inv);
+    }
+    if (threadIdx.x == 0) c.scales[tile] = m / kF8Top;
 }
 
 template <typename T>
@@ -172,88 +237,118 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// One thread per eight codes of a row.
-template <typename T, bool VEC>
+// One thread per 16 codes of a row, kGroups of them at once.
+template <typename T, bool VEC, typename I>
 __global__ void __launch_bounds__(256) f8_decode_kernel(F8Codec c) {
-    const int64_t nb = (c.ne0 + kF8Block - 1) / kF8Block, rb = (c.n_rows + c.block_rows - 1) / c.block_rows;
-    const int64_t ng = (c.ne0 + 7) / 8, total = c.n_mats * c.n_rows * ng;
-    for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < total; u += (int64_t)gridDim.x * 256) {
-        const int64_t row = u / ng, col = (u - row * ng) * 8;
-        const int64_t mat = row / c.n_rows, r = row - mat * c.n_rows;
-        const float s = __ldg(c.scales + (mat * rb + r / c.block_rows) * nb + col / kF8Block);
-        const uint8_t *p = c.codes + mat * c.code_mat_stride + r * c.code_row_stride + col;
-        const int n = c.ne0 - col < 8 ? (int)(c.ne0 - col) : 8;
-        uint16_t q[4] = {0, 0, 0, 0};
-        if (n == 8) {
-            const uint2 w = __ldg(reinterpret_cast<const uint2 *>(p));
-            q[0] = (uint16_t)w.x;
-            q[1] = (uint16_t)(w.x >> 16);
-            q[2] = (uint16_t)w.y;
-            q[3] = (uint16_t)(w.y >> 16);
-        } else {
-            for (int i = 0; i < n; i++) q[i >> 1] |= (uint16_t)((uint16_t)p[i] << (8 * (i & 1)));
-        }
-        __align__(16) T y[8];
+    constexpr int kGroups = 2;
+    const I nb = (I)((c.ne0 + kF8Block - 1) / kF8Block), rows = (I)c.n_rows;
+    const int64_t rb = (c.n_rows + c.block_rows - 1) / c.block_rows;
+    const I ng = (I)((c.ne0 + kElems - 1) / kElems), total = (I)(c.n_mats * c.n_rows) * ng;
+    const int shift = c.block_rows == 1 ? 0 : 7;
+    const I u0 = (I)blockIdx.x * (256 * kGroups) + threadIdx.x;
+    uint32_t q[kGroups][4];
+    float s[kGroups];
+    int n[kGroups];
+    int64_t at[kGroups];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float2 f = e4m3x2_val(q[i]);
-            y[2 * i] = from_f32<T>(f.x * s);
-            y[2 * i + 1] = from_f32<T>(f.y * s);
-        }
-        T *o = static_cast<T *>(c.dst) + row * c.ne0 + col;
-        if (VEC && n == 8) {
-#pragma unroll
-            for (int i = 0; i < (int)sizeof(T) / 2; i++)
-                reinterpret_cast<uint4 *>(o)[i] = reinterpret_cast<const uint4 *>(y)[i];
+    for (int k = 0; k < kGroups; k++) {
+        const I u = u0 + (I)(k * 256);
+        n[k] = 0;
+        if (u >= total) continue;
+        const I g = u / ng, b = u - g * ng;
+        const I mat = c.n_mats > 1 ? g / rows : 0, r = g - mat * rows;
+        const int64_t col = (int64_t)b * kElems;
+        s[k] = __ldg(c.scales + ((int64_t)mat * rb + (int64_t)(r >> shift)) * (int64_t)nb + (int64_t)(b >> 3));
+        n[k] = c.ne0 - col < kElems ? (int)(c.ne0 - col) : kElems;
+        at[k] = (int64_t)g * c.ne0 + col;
+        const uint8_t *p = c.codes + (int64_t)mat * c.code_mat_stride + (int64_t)r * c.code_row_stride + col;
+        if (n[k] == kElems) {
+            const uint4 w = __ldcs(reinterpret_cast<const uint4 *>(p));
+            q[k][0] = w.x;
+            q[k][1] = w.y;
+            q[k][2] = w.z;
+            q[k][3] = w.w;
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (i < n) o[i] = y[i];
+            for (int i = 0; i < 4; i++) q[k][i] = 0;
+#pragma unroll
+            for (int i = 0; i < kElems; i++)
+                if (i < n[k]) q[k][i >> 2] |= (uint32_t)p[i] << (8 * (i & 3));
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kGroups; k++) {
+        __align__(16) T y[kElems];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float2 f = e4m3x2_val((uint16_t)(q[k][i >> 1] >> (16 * (i & 1))));
+            y[2 * i] = from_f32<T>(f.x * s[k]);
+            y[2 * i + 1] = from_f32<T>(f.y * s[k]);
+        }
+        T *o = static_cast<T *>(c.dst) + at[k];
+        if (VEC && n[k] == kElems) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T); i++) reinterpret_cast<uint4 *>(o)[i] = reinterpret_cast<const uint4 *>(y)[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < kElems; i++)
+                if (i < n[k]) o[i] = y[i];
         }
     }
 }
 
-unsigned grid_for(int64_t items, int64_t per_block, int num_sms, int waves) {
-    int64_t b = (items + per_block - 1) / per_block;
-    const int64_t most = (int64_t)num_sms * waves;
-    return (unsigned)(b < 1 ? 1 : b > most ? most : b);
+// Thread blocks for `items` of `per_block`; 0 where no grid holds them.
+unsigned grid_for(int64_t items, int64_t per_block) {
+    const int64_t b = (items + per_block - 1) / per_block;
+    return b > INT32_MAX ? 0 : (unsigned)b;
+}
+
+template <int ST, bool VEC>
+cudaError_t encode(const F8Codec &c, cudaStream_t st) {
+    const int64_t nb = (c.ne0 + kF8Block - 1) / kF8Block;
+    if (c.block_rows != 1) {
+        const unsigned g = grid_for(c.n_mats * ((c.n_rows + kF8Block - 1) / kF8Block) * nb, 1);
+        if (!g) return cudaErrorInvalidValue;
+        f8_encode_tiles_kernel<ST, VEC><<<g, 256, 0, st>>>(c);
+        return cudaGetLastError();
+    }
+    const int64_t total = c.n_mats * c.n_rows * nb;
+    const unsigned g = grid_for(total, 256 / kLanes * units<ST>());
+    if (!g) return cudaErrorInvalidValue;
+    if (total < INT32_MAX) f8_encode_rows_kernel<ST, VEC, uint32_t><<<g, 256, 0, st>>>(c);
+    else f8_encode_rows_kernel<ST, VEC, uint64_t><<<g, 256, 0, st>>>(c);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t decode(const F8Codec &c, bool vec, cudaStream_t st) {
+    const int64_t total = c.n_mats * c.n_rows * ((c.ne0 + kElems - 1) / kElems);
+    const unsigned g = grid_for(total, 512);
+    if (!g) return cudaErrorInvalidValue;
+    if (total >= INT32_MAX) f8_decode_kernel<T, false, uint64_t><<<g, 256, 0, st>>>(c);
+    else if (vec) f8_decode_kernel<T, true, uint32_t><<<g, 256, 0, st>>>(c);
+    else f8_decode_kernel<T, false, uint32_t><<<g, 256, 0, st>>>(c);
+    return cudaGetLastError();
 }
 
 }  // namespace
 
-cudaError_t launch_f8_encode(const F8Codec &c, int num_sms, cudaStream_t st) {
+cudaError_t launch_f8_encode(const F8Codec &c, cudaStream_t st) {
     const int64_t esz = c.type == SHC_SRC_F32 ? 4 : 2;
     // 128-bit loads where every row starts on a 16-byte boundary
     const bool vec = ((uintptr_t)c.src & 15) == 0 && c.src_row_stride * esz % 16 == 0 &&
                      c.src_mat_stride * esz % 16 == 0;
-    const int64_t nb = (c.ne0 + kF8Block - 1) / kF8Block;
-    if (c.block_rows == 1) {
-        const unsigned g = grid_for(c.n_mats * c.n_rows * nb, 256 / kLanes, num_sms, 64);
-        if (vec) f8_encode_rows_kernel<true><<<g, 256, 0, st>>>(c);
-        else f8_encode_rows_kernel<false><<<g, 256, 0, st>>>(c);
-    } else {
-        const unsigned g = grid_for(c.n_mats * ((c.n_rows + kF8Block - 1) / kF8Block) * nb, 1, num_sms, 64);
-        if (vec) f8_encode_tiles_kernel<true><<<g, 256, 0, st>>>(c);
-        else f8_encode_tiles_kernel<false><<<g, 256, 0, st>>>(c);
-    }
-    return cudaGetLastError();
+    if (c.type == SHC_SRC_F32) return vec ? encode<SHC_SRC_F32, true>(c, st) : encode<SHC_SRC_F32, false>(c, st);
+    if (c.type == SHC_SRC_F16) return vec ? encode<SHC_SRC_F16, true>(c, st) : encode<SHC_SRC_F16, false>(c, st);
+    return vec ? encode<SHC_SRC_BF16, true>(c, st) : encode<SHC_SRC_BF16, false>(c, st);
 }
 
-cudaError_t launch_f8_decode(const F8Codec &c, int num_sms, cudaStream_t st) {
+cudaError_t launch_f8_decode(const F8Codec &c, cudaStream_t st) {
     const int64_t esz = c.type == SHC_SRC_F32 ? 4 : 2;
     const bool vec = ((uintptr_t)c.dst & 15) == 0 && c.ne0 * esz % 16 == 0;
-    const unsigned g = grid_for(c.n_mats * c.n_rows * ((c.ne0 + 7) / 8), 256, num_sms, 64);
-    if (c.type == SHC_SRC_F32) {
-        if (vec) f8_decode_kernel<float, true><<<g, 256, 0, st>>>(c);
-        else f8_decode_kernel<float, false><<<g, 256, 0, st>>>(c);
-    } else if (c.type == SHC_SRC_F16) {
-        if (vec) f8_decode_kernel<__half, true><<<g, 256, 0, st>>>(c);
-        else f8_decode_kernel<__half, false><<<g, 256, 0, st>>>(c);
-    } else {
-        if (vec) f8_decode_kernel<__nv_bfloat16, true><<<g, 256, 0, st>>>(c);
-        else f8_decode_kernel<__nv_bfloat16, false><<<g, 256, 0, st>>>(c);
-    }
-    return cudaGetLastError();
+    if (c.type == SHC_SRC_F32) return decode<float>(c, vec, st);
+    if (c.type == SHC_SRC_F16) return decode<__half>(c, vec, st);
+    return decode<__nv_bfloat16>(c, vec, st);
 }
 
 }  // namespace shc

@@ -29,8 +29,8 @@ struct F8Codec {
     int64_t n_mats, n_rows, ne0;
     int block_rows;  // 1 or kF8Block
 };
-cudaError_t launch_f8_encode(const F8Codec &c, int num_sms, cudaStream_t st);
-cudaError_t launch_f8_decode(const F8Codec &c, int num_sms, cudaStream_t st);
+cudaError_t launch_f8_encode(const F8Codec &c, cudaStream_t st);
+cudaError_t launch_f8_decode(const F8Codec &c, cudaStream_t st);
 
 // D = A W^T (W [n, k], A [rows, k]) or, transposed, D = A W (A [rows, n]).
 struct F8Product {

@@ -26,7 +26,7 @@ class CpuContext(sh.Context):
     def _f8_here(self, t, what):
         pass
 
-    def _stream(self, stream):
+    def _f8_stream(self):
         return None
 
 
