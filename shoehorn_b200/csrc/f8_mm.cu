@@ -33,20 +33,35 @@
 namespace shc {
 namespace {
 
-constexpr int kTileM = 128;
-constexpr int kTileK = kF8Block;  // bytes of one stage row, the swizzle's width
+constexpr int kTileM = 128;           // rows of one CTA's tile
+constexpr int kTileK = kF8Block;      // bytes of one stage row, the swizzle's width
+constexpr int kMmaK = 32;             // contraction length of one tcgen05 product of 8-bit operands
+constexpr int kSlotBlocks = 4;        // contraction blocks whose scales share a slot
+constexpr int kSlots = 3;             // of scales on their way
+constexpr int kPieceBytes = 32 * 64;  // a warp's staging of 32 output rows x 64 bytes
 constexpr unsigned long long kWaitNs = 4000000000ull;
-constexpr int kMmaK = 32;  // contraction length of one tcgen05 product of 8-bit operands
+constexpr unsigned long long kSettleNs = 2000000ull;
 
-template <int BN>
+// BN output columns per tile; PAIR CTAs (a cluster of one or two) work on one
+// tile of PAIR x 128 rows.
+template <int BN, int PAIR>
 struct Shape {
-    static constexpr int kStages = BN == 128 ? 6 : 4;
-    static constexpr int kABytes = kTileM * kTileK, kBBytes = BN * kTileK;
+    static constexpr int kBRows = BN / PAIR;  // rows of B that one CTA holds
+    static constexpr int kABytes = kTileM * kTileK, kBBytes = kBRows * kTileK;
     static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kEpiWarps = BN / 32;  // four per 128 columns, one per 32 TMEM lanes
-    static constexpr int kThreads = (kEpiWarps + 2) * 32;
-    static constexpr size_t kSmem = (size_t)kStages * kStageBytes + 1024;  // + alignment of the ring
-    static constexpr uint32_t kTmemCols = 2 * BN;
+    static constexpr int kStages = 163840 / kStageBytes;  // 160 KB
+    static constexpr int kEpiWarps = 8;                   // two for each 32 TMEM lanes
+    static constexpr int kThreads = (kEpiWarps + 4) * 32;
+    // All of TMEM: each 128-column half of the tile has accumulators of its
+    // own, so the epilogue drains one half while the other is summed.
+    static constexpr int kHalves = BN / 128;
+    static constexpr int kBufs = 512 / BN;
+    static_assert(kBufs < kStages, "see the order of the product warps' waits");
+    static constexpr int kGroups = BN / 128;  // groups of 64 columns that one epilogue warp drains
+    static constexpr int kAtOnce = BN == 128 ? 4 : 1;  // 16-column TMEM loads in flight, as registers allow
+    static constexpr int kSlotBytes = kSlotBlocks * BN * 4;  // [block][BN / 128][128 rows]
+    static constexpr size_t kSmem =
+        (size_t)kStages * kStageBytes + kEpiWarps * kPieceBytes + kSlots * kSlotBytes + 1024;  // + alignment
 };
 
 struct MmArgs {
@@ -54,7 +69,7 @@ struct MmArgs {
     const float *w_scales;
     const void *offsets;
     int offsets_64;
-    int64_t n_rows, n_experts;
+    int n_rows, n_experts;
     int64_t a_scale_stride;
     int64_t w_scale_expert, w_scale_out, w_scale_in;  // strides of a tile's scale: expert, output block, contraction block
     int out;       // output columns
@@ -63,40 +78,74 @@ struct MmArgs {
     void *dst;
     int64_t dst_row_stride;
     int dst_type;
-    int vec;  // 16-byte stores of whole 8-column groups
+    int vec;        // rows of dst start on 16-byte boundaries
+    int tma_store;  // map_d describes dst
     int *status;
 };
 
 struct Control {
-    unsigned long long full[8], empty[8];
-    unsigned long long acc_full[2], acc_empty[2];
-    unsigned long long drain;
+    unsigned long long full[5];    // a stage's bytes have landed
+    unsigned long long done[5];    // its products are done: it is free
+    struct {
+        unsigned long long full, empty;  // an accumulator holds a block's sums; they have been read
+    } acc[2][4];  // [half][buffer]
+    unsigned long long slot_full[kSlots], slot_empty[kSlots];
+    unsigned long long drain[2];
+    int4 slot[kSlots];  // what a slot's scales are for: first row of this CTA, end of rows, first column, blocks (see kLast)
     uint32_t tmem;
     int abort;
 };
+constexpr int kLast = 256;  // added to a slot's blocks where they are the tile's last ones
 
 // ---------------------------------------------------------------- waits
 
-// True when the phase completed, false after kWaitNs or once another warp gave up.
-__device__ __noinline__ bool wait_slow(unsigned long long *b, uint32_t parity, volatile int *abort, int *status) {
-    const unsigned long long t0 = global_ns();
-    while (!mbar_test(b, parity)) {
+__device__ __forceinline__ bool bar_test(unsigned long long *b, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(smem_u32(b)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// True when the phase completed, false after kWaitNs or once another warp gave
+// up.  The clock is read on every 256th try only: reading it takes longer than
+// most waits.  (Inline: a call would spill the epilogue's sums.)
+__device__ __forceinline__ bool bar_wait(unsigned long long *b, uint32_t parity, volatile int *abort, int *status) {
+    unsigned long long t0 = 0;
+#pragma unroll 1
+    for (uint32_t i = 1;; i++) {
+        if (bar_test(b, parity)) return true;
+        if (i % 256) continue;
         if (*abort) return false;
-        if (global_ns() - t0 > kWaitNs) {
+        const unsigned long long t = global_ns();
+        if (t0 == 0) t0 = t;
+        if (t - t0 > kWaitNs) {
             *abort = 1;
             set_status(status, SHC_ETIMEOUT);
             return false;
         }
     }
-    return true;
 }
-__device__ __forceinline__ bool bar_wait(unsigned long long *b, uint32_t parity, volatile int *abort, int *status) {
-    return mbar_test(b, parity) || wait_slow(b, parity, abort, status);
+// One lane of a converged warp, known to the compiler to be one (so that what
+// it alone executes can be kept in uniform registers, which tcgen05 needs).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(one));
+    return one != 0;
+}
+// For a whole warp: one try by all lanes, then one lane waits for all (32
+// pollers a barrier slow the others down).
+__device__ __forceinline__ bool warp_wait(unsigned long long *b, uint32_t parity, volatile int *abort, int *status) {
+    if (__all_sync(~0u, bar_test(b, parity))) return true;
+    int ok = 1;
+    if ((threadIdx.x & 31) == 0) ok = bar_wait(b, parity, abort, status);
+    return __shfl_sync(~0u, ok, 0);
 }
 // After a give-up: wait, bounded, for work that is still in flight.
-__device__ __noinline__ void wait_drain(unsigned long long *b, uint32_t parity) {
+__device__ __noinline__ void wait_drain(unsigned long long *b, uint32_t parity, unsigned long long limit_ns) {
     const unsigned long long t0 = global_ns();
-    while (!mbar_test(b, parity) && global_ns() - t0 < kWaitNs) {
+    while (!bar_test(b, parity) && global_ns() - t0 < limit_ns) {
     }
 }
 __device__ __forceinline__ void expect_tx(unsigned long long *b, uint32_t bytes) {
@@ -105,17 +154,72 @@ __device__ __forceinline__ void expect_tx(unsigned long long *b, uint32_t bytes)
 
 // ---------------------------------------------------------------- TMA, tcgen05
 
-__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, unsigned long long *bar, int x, int y) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
-        "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y)
-        : "memory");
+// Loads signal `bar`, an address in the cluster's shared window: the CTA's
+// own barrier, or in a pair the leader's.
+template <int PAIR>
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y) {
+    if (PAIR == 2)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+            "l"(map), "r"(bar), "r"(x), "r"(y)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+            "l"(map), "r"(bar), "r"(x), "r"(y)
+            : "memory");
 }
-__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap *map, unsigned long long *bar, int x, int y, int z) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
-        "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
-        : "memory");
+template <int PAIR>
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z) {
+    if (PAIR == 2)
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+            "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+            "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+            : "memory");
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, uint32_t src, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src),
+                 "r"(x), "r"(y)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// This thread's stores have read their shared memory / are complete.
+__device__ __forceinline__ void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+// The same shared address in the leader CTA of the pair.
+__device__ __forceinline__ uint32_t in_leader(uint32_t addr) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+    return r;
+}
+// Arrives on a barrier of this CTA or, in a pair, of the leader.  (What is
+// handed over is TMEM, ordered by tcgen05.fence; a release at cluster scope
+// would wait for the warp's outstanding memory operations: 1150 cycles a
+// block.)
+template <int PAIR>
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+    if (PAIR == 2) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+template <int PAIR>
+__device__ __forceinline__ void sync_all() {
+    if (PAIR == 2) {
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    } else {
+        __syncthreads();
+    }
 }
 
 // Shared-memory descriptor of a 128-byte-swizzled operand tile.  stride: from
@@ -126,90 +230,97 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead, uint
            (1ull << 46) | (2ull << 61);
 }
 // Instruction descriptor: E4M3 operands, f32 accumulator, A K-major.
-__host__ __device__ constexpr uint32_t instr_desc(int n, bool b_mn_major) {
-    return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24);
+__host__ __device__ constexpr uint32_t instr_desc(int m, int n, bool b_mn_major) {
+    return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
+template <int PAIR>
 __device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
-        : "memory");
+    if (PAIR == 2)
+        asm volatile(
+            "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+            " tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+            : "memory");
+    else
+        asm volatile(
+            "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+            " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+            : "memory");
 }
+// Arrives on the barrier (in a pair: on both CTAs' barriers at this address)
+// when the products issued so far are done.
+template <int PAIR>
 __device__ __forceinline__ void mma_commit(unsigned long long *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
+    if (PAIR == 2)
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                smem_u32(bar)),
+            "h"((uint16_t)3)
+            : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                     : "memory");
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// 32 consecutive f32 columns of the warp's 32 TMEM lanes, one lane per thread.
-__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t r[32]) {
+// 16 consecutive f32 columns of the warp's 32 TMEM lanes, one lane per thread.
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t r[16]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(addr));
 }
 // Waits for this thread's TMEM loads; r is tied to the wait so that no use of
 // it moves ahead.
-__device__ __forceinline__ void tmem_wait_ld(uint32_t r[32]) {
+__device__ __forceinline__ void tmem_wait_ld(uint32_t r[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
                  : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
-                   "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
-                   "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27])
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
                  :
                  : "memory");
-    asm volatile("" : "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
-}
-
-// acc += part * (s, s), two f32 fused multiply-adds per instruction.
-__device__ __forceinline__ void fma2(uint64_t &acc, uint32_t p0, uint32_t p1, uint64_t s2) {
-    asm("{\n .reg .b64 t;\n mov.b64 t, {%1, %2};\n fma.rn.f32x2 %0, t, %3, %0;\n}" : "+l"(acc) : "r"(p0), "r"(p1), "l"(s2));
 }
 
 // ---------------------------------------------------------------- tiles
 
 struct Tile {
-    int64_t expert, row0, row_end;  // rows [row0, min(row0 + 128, row_end)) of A and D
-    int col0;                       // first output column
+    int expert, row0, row_end;  // rows [row0, min(row0 + TM, row_end)) of A and D
+    int col0;                   // first output column
 };
 
-// Hands out the tiles of the grid's CTAs in turn: expert by expert, within an
+// Hands out tiles of TM x BN to the grid's CTAs (or pairs) in turn: expert by expert, within an
 // expert a column of row tiles before the next column (so CTAs running
 // together share W's tiles in L2).  Called by whole warps; experts are looked
 // up 32 at a time.  Offsets are clamped to the rows there are, so no tile
 // reaches outside A and D whatever they hold.
+template <int BN, int PAIR>
 struct Tiles {
-    int64_t t, base, e0;  // base: tiles before expert e0
-    int64_t n_out, step;
+    static constexpr int TM = kTileM * PAIR;
+    int64_t t, base;  // base: tiles before expert e0
+    int e0;
     const MmArgs &p;
-    __device__ Tiles(const MmArgs &args, int bn)
-        : t(blockIdx.x), base(0), e0(0), n_out((args.out + bn - 1) / bn), step(gridDim.x), p(args) {}
-    __device__ __forceinline__ int64_t offset(int64_t e) const {
+    __device__ __forceinline__ Tiles(const MmArgs &args) : t(blockIdx.x / PAIR), base(0), e0(0), p(args) {}
+    __device__ __forceinline__ int offset(int e) const {
         const int64_t v = p.offsets_64 ? static_cast<const int64_t *>(p.offsets)[e]
                                        : (int64_t) static_cast<const int32_t *>(p.offsets)[e];
-        return v < 0 ? 0 : v > p.n_rows ? p.n_rows : v;
+        return v < 0 ? 0 : v > p.n_rows ? p.n_rows : (int)v;
     }
-    __device__ bool next(Tile &o, int bn) {
+    __device__ __forceinline__ bool next(Tile &o) {
         const int lane = threadIdx.x & 31;
+        const int n_out = (p.out + BN - 1) / BN;
         for (;;) {
             if (e0 >= p.n_experts) return false;
-            int64_t lo = 0, hi = p.n_rows;
-            const int64_t e = e0 + lane;
+            int lo = 0, hi = lane ? 0 : p.n_rows;
             if (p.offsets) {
+                const int e = e0 + lane;
                 lo = e < p.n_experts ? offset(e) : 0;
                 hi = e < p.n_experts ? offset(e + 1) : 0;
-            } else if (lane) {
-                hi = 0;
             }
             if (hi < lo) hi = lo;
-            const int64_t mine = (hi - lo + kTileM - 1) / kTileM * n_out;
+            const int64_t mine = (int64_t)(((uint32_t)(hi - lo) + TM - 1) / TM) * n_out;
             int64_t sum = mine;  // inclusive prefix sum over the lanes
             for (int d = 1; d < 32; d <<= 1) {
                 const int64_t v = __shfl_up_sync(~0u, sum, d);
@@ -218,14 +329,15 @@ struct Tiles {
             const unsigned in = __ballot_sync(~0u, t < base + sum);
             if (in) {
                 const int l = __ffs(in) - 1;
-                const int64_t first = base + __shfl_sync(~0u, sum - mine, l);
-                const int64_t elo = __shfl_sync(~0u, lo, l), ehi = __shfl_sync(~0u, hi, l);
-                const int64_t at = t - first, mt = (ehi - elo + kTileM - 1) / kTileM;
+                const uint32_t at = (uint32_t)(t - base - __shfl_sync(~0u, sum - mine, l));  // below 2^31: one expert's tiles
+                lo = __shfl_sync(~0u, lo, l);
+                hi = __shfl_sync(~0u, hi, l);
+                const uint32_t mt = ((uint32_t)(hi - lo) + TM - 1) / TM, ct = at / mt;
                 o.expert = e0 + l;
-                o.col0 = (int)(at / mt) * bn;
-                o.row0 = elo + at % mt * kTileM;
-                o.row_end = ehi;
-                t += step;
+                o.col0 = (int)ct * BN;
+                o.row0 = lo + (int)(at - ct * mt) * TM;
+                o.row_end = hi;
+                t += gridDim.x / PAIR;
                 return true;
             }
             base += __shfl_sync(~0u, sum, 31);
@@ -236,208 +348,375 @@ struct Tiles {
 
 // ---------------------------------------------------------------- epilogue stores
 
-__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
+__device__ __forceinline__ uint32_t pack_f16(float2 v) {
+    const __half2 h = __floats2half2_rn(v.x, v.y);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
-__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+__device__ __forceinline__ uint32_t pack_bf16(float2 v) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// Eight consecutive columns of one row of D.
-__device__ __forceinline__ void store8(const MmArgs &p, int64_t row, int col, const float v[8]) {
-    const int64_t at = row * p.dst_row_stride + col;
-    if (p.dst_type == SHC_SRC_F32) {
-        float *d = static_cast<float *>(p.dst) + at;
-        if (p.vec && col + 8 <= p.out) {
-            reinterpret_cast<float4 *>(d)[0] = make_float4(v[0], v[1], v[2], v[3]);
-            reinterpret_cast<float4 *>(d)[1] = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
+// A warp's 32 x 64 sums (lane = row) to D, 64 bytes of each row at a time
+// through `stage` (32 rows x 64 bytes, 16-byte pieces swizzled as TMA's
+// 64-byte mode does, so both sides are free of bank conflicts): by one TMA
+// store where all 32 rows may be written, else row by row.
+template <int DT>
+__device__ __forceinline__ void store_rows(const MmArgs &p, const CUtensorMap *map_d, uint32_t stage, const float2 acc[32],
+                                           int row0, int row_end, int col0) {
+    constexpr int esz = DT == SHC_SRC_F32 ? 4 : 2;
+    constexpr int kCols = 64 / esz;  // columns of 64 bytes
+    constexpr int kPer = 16 / esz;   // columns of 16 bytes
+    const int lane = threadIdx.x & 31;
+    // rows past the end may be written only where TMA clips them
+    const bool tma = p.tma_store && (row0 + 32 <= row_end || row_end == p.n_rows);
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (col + i < p.out) d[i] = v[i];
+    for (int q = 0; q < 64 / kCols; q++) {
+        const int col = col0 + q * kCols;
+        if (col >= p.out) break;
+        if (lane == 0) store_wait_read();  // the piece before this one has left the stage
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float2 *v = acc + (q * kCols + k * kPer) / 2;
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (DT == SHC_SRC_F32) w[i] = __float_as_uint(i & 1 ? v[i / 2].y : v[i / 2].x);
+                else w[i] = DT == SHC_SRC_F16 ? pack_f16(v[i % (kPer / 2)]) : pack_bf16(v[i % (kPer / 2)]);
+            }
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 64 + ((k ^ (lane >> 1 & 3)) << 4)),
+                         "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                         : "memory");
         }
-        return;
-    }
-    uint16_t *d = static_cast<uint16_t *>(p.dst) + at;
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-        w[i] = p.dst_type == SHC_SRC_F16 ? pack_f16(v[2 * i], v[2 * i + 1]) : pack_bf16(v[2 * i], v[2 * i + 1]);
-    if (p.vec && col + 8 <= p.out) {
-        *reinterpret_cast<uint4 *>(d) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (col + i < p.out) d[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+        if (tma) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) tma_store_2d(map_d, stage, col, row0);
+            continue;
+        }
+        __syncwarp();
+        const int rows = row_end - row0 < 32 ? row_end - row0 : 32;
+        uint8_t *d = static_cast<uint8_t *>(p.dst) + ((int64_t)row0 * p.dst_row_stride + col) * esz;
+        const int64_t pitch = p.dst_row_stride * esz;
+        if (p.vec && col + kCols <= p.out) {
+            for (int r = lane >> 2; r < rows; r += 8) {
+                uint32_t w[4];
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                             : "r"(stage + r * 64 + (((lane & 3) ^ (r >> 1 & 3)) << 4)));
+                *reinterpret_cast<uint4 *>(d + r * pitch + (lane & 3) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        } else {
+            // kCols columns of 32 / kCols rows at once
+            const int c = lane % kCols;
+            if (col + c < p.out) {
+                for (int r = lane / kCols; r < rows; r += 32 / kCols) {
+                    const uint32_t at = stage + r * 64 + ((((c / kPer) ^ (r >> 1 & 3)) << 4) | (c % kPer) * esz);
+                    if (DT == SHC_SRC_F32) {
+                        uint32_t v;
+                        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at));
+                        *reinterpret_cast<uint32_t *>(d + r * pitch + c * 4) = v;
+                    } else {
+                        uint16_t v;
+                        asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(at));
+                        *reinterpret_cast<uint16_t *>(d + r * pitch + c * 2) = v;
+                    }
+                }
+            }
+        }
+        __syncwarp();
     }
 }
 
 // ---------------------------------------------------------------- kernel
 
-template <int BN, bool TRANS>
-__global__ void __launch_bounds__(Shape<BN>::kThreads, 1)
+template <int BN, int PAIR, bool TRANS>
+__global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1)
     f8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
-                      const __grid_constant__ MmArgs p) {
-    using S = Shape<BN>;
+                      const __grid_constant__ CUtensorMap map_d, const __grid_constant__ MmArgs p) {
+    using S = Shape<BN, PAIR>;
     extern __shared__ uint8_t smem_raw[];
     __shared__ Control ctl;
     const uint32_t ring = (smem_u32(smem_raw) + 1023) & ~1023u;  // the swizzle's pattern repeats every 1024 bytes
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    const int rank = PAIR == 2 ? (int)cluster_rank() : 0;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; s++) {
             mbar_init(&ctl.full[s], 1);
-            mbar_init(&ctl.empty[s], 1);
+            mbar_init(&ctl.done[s], 1);
         }
-        for (int i = 0; i < 2; i++) {
-            mbar_init(&ctl.acc_full[i], 1);
-            mbar_init(&ctl.acc_empty[i], S::kEpiWarps);
+        for (int h = 0; h < S::kHalves; h++)
+            for (int i = 0; i < S::kBufs; i++) {
+                mbar_init(&ctl.acc[h][i].full, 1);
+                mbar_init(&ctl.acc[h][i].empty, S::kEpiWarps / S::kHalves * PAIR);
+            }
+        for (int i = 0; i < kSlots; i++) {
+            mbar_init(&ctl.slot_full[i], 1);
+            mbar_init(&ctl.slot_empty[i], S::kEpiWarps);
         }
-        mbar_init(&ctl.drain, 1);
+        for (int i = 0; i < 2; i++) mbar_init(&ctl.drain[i], 1);
         ctl.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == S::kEpiWarps) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem)),
-                     "n"(S::kTmemCols)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        if (PAIR == 2) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem)), "n"(512)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem)), "n"(512)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        }
     }
     fence_before();
     __syncthreads();
+    if (PAIR == 2) sync_all<PAIR>();  // both CTAs' barriers are set up
     fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&ctl.tmem);
     volatile int *abort = &ctl.abort;
 
-    Tiles tiles(p, BN);
-    Tile tile;
-    if (warp == S::kEpiWarps) {
-        // ------------------------------------------------ loads
-        uint32_t it = 0;
-        bool ok = true;
-        while (ok && tiles.next(tile, BN)) {
-            const int64_t rows = tile.row_end - tile.row0 < kTileM ? tile.row_end - tile.row0 : kTileM;
-            const int boxes = (int)((rows + p.a_box - 1) / p.a_box);
-            if (lane == 0) {
-                for (int c = 0; ok && c < p.blocks_c; c++) {
-                    const uint32_t s = it % S::kStages, round = it / S::kStages;
-                    if (!bar_wait(&ctl.empty[s], (round & 1) ^ 1, abort, p.status)) {
-                        ok = false;
-                        break;
-                    }
-                    const uint32_t a = ring + s * S::kStageBytes, b = a + S::kABytes;
-                    expect_tx(&ctl.full[s], boxes * p.a_box * kTileK + S::kBBytes);
-                    for (int i = 0; i < boxes; i++)
-                        tma_2d(a + i * p.a_box * kTileK, &map_a, &ctl.full[s], c * kTileK, (int)tile.row0 + i * p.a_box);
+    const uint32_t stages = ring + S::kStages * S::kStageBytes;  // of the epilogue, then the slots of scales
+    float *const slots = reinterpret_cast<float *>(smem_raw + (stages - smem_u32(smem_raw)) + S::kEpiWarps * kPieceBytes);
+    if (warp >= S::kEpiWarps) {
+        Tiles<BN, PAIR> tiles(p);
+        Tile tile;
+        if (warp == S::kEpiWarps) {
+            // ------------------------------------------------ loads
+            uint32_t it = 0;
+            bool ok = true;
+            while (ok && tiles.next(tile)) {
+                int boxes[PAIR];  // of A, for each CTA
 #pragma unroll
-                    for (int j = 0; j < BN / 128; j++) {
-                        const int o = tile.col0 + j * 128, x = c * kTileK;
-                        tma_3d(b + j * 128 * kTileK, &map_w, &ctl.full[s], TRANS ? o : x, TRANS ? x : o, (int)tile.expert);
+                for (int r = 0; r < PAIR; r++) {
+                    int rows = tile.row_end - tile.row0 - r * kTileM;
+                    rows = rows < 0 ? 0 : rows > kTileM ? kTileM : rows;
+                    boxes[r] = (rows + p.a_box - 1) / p.a_box;
+                }
+                const int mine = PAIR == 2 && rank ? boxes[PAIR - 1] : boxes[0];
+                uint32_t bytes = 0;
+#pragma unroll
+                for (int r = 0; r < PAIR; r++) bytes += boxes[r] * p.a_box * kTileK + S::kBBytes;
+                if (elect_one()) {
+                    for (int c = 0; c < p.blocks_c; c++) {
+                        const uint32_t s = it % S::kStages, round = it / S::kStages;
+                        if (!bar_wait(&ctl.done[s], (round & 1) ^ 1, abort, p.status)) {
+                            ok = false;
+                            break;
+                        }
+                        const uint32_t a = ring + s * S::kStageBytes, b = a + S::kABytes;
+                        uint32_t bar = smem_u32(&ctl.full[s]);
+                        if (rank == 0) expect_tx(&ctl.full[s], bytes);  // the leader counts both CTAs' bytes
+                        if (PAIR == 2) bar = in_leader(bar);
+                        for (int i = 0; i < mine; i++)
+                            tma_2d<PAIR>(a + i * p.a_box * kTileK, &map_a, bar, c * kTileK,
+                                         tile.row0 + rank * kTileM + i * p.a_box);
+#pragma unroll
+                        for (int j = 0; j < S::kBRows / 128; j++) {
+                            const int o = tile.col0 + rank * S::kBRows + j * 128, x = c * kTileK;
+                            tma_3d<PAIR>(b + j * 128 * kTileK, &map_w, bar, TRANS ? o : x, TRANS ? x : o, tile.expert);
+                        }
+                        it++;
                     }
-                    it++;
+                }
+                ok = __all_sync(~0u, (int)ok);
+            }
+            it = __reduce_max_sync(~0u, it);
+            if (lane == 0 && !ok) {  // copies still in flight land before the CTA ends
+                if (rank == 0)
+                    for (uint32_t k = it > S::kStages ? it - S::kStages : 0; k < it; k++)
+                        wait_drain(&ctl.full[k % S::kStages], (k / S::kStages) & 1, kWaitNs);
+                else  // these signal the other CTA's barriers
+                    wait_drain(&ctl.drain[0], 0, kSettleNs);
+            }
+        } else if (warp < S::kEpiWarps + 3) {
+            // ------------------------------------------------ products (of a pair: issued by its leader)
+            // Every block's sum starts afresh in its own accumulator, so two
+            // warps issue the even and the odd blocks without regard to one
+            // another; one thread's waits and issues take longer than a
+            // block's products.
+            const uint32_t me = warp - (S::kEpiWarps + 1);
+            constexpr uint32_t idesc = instr_desc(kTileM * PAIR, 128, TRANS);
+            const uint64_t da0 = smem_desc(ring, 16, 1024);
+            const uint64_t db0 = TRANS ? smem_desc(ring + S::kABytes, 128 * kTileK, 1024) : smem_desc(ring + S::kABytes, 16, 1024);
+            // the next 32 of the contraction: MN-major 32 rows of 128 columns further, K-major 32 bytes along the row
+            constexpr uint64_t kStepA = kMmaK >> 4, kStepB = (TRANS ? kMmaK * 128 : kMmaK) >> 4;
+            // The half's columns of B.  A CTA of a pair holds 128 adjacent columns, 64 of either half.
+            constexpr uint64_t kHalfB = (TRANS && PAIR == 2 ? 64 : 128 / PAIR * kTileK) >> 4;
+            uint32_t it = me, s = me, phase = 0;  // this warp's block, counted over all tiles; its stage
+            uint32_t first = me;                  // its first block in the tile
+            bool ok = rank == 0;
+            while (ok && tiles.next(tile)) {
+                if (elect_one()) {
+                    for (uint32_t c = first; c < (uint32_t)p.blocks_c; c += 2, it += 2) {
+                        const uint32_t buf = it % S::kBufs, acc_phase = ((it / S::kBufs) & 1) ^ 1;
+                        const uint64_t da = da0 + (uint64_t)(s * (S::kStageBytes >> 4)), db = db0 + (uint64_t)(s * (S::kStageBytes >> 4));
+#pragma unroll
+                        for (int h = 0; h < S::kHalves; h++) {
+                            ok = bar_wait(&ctl.acc[h][buf].empty, acc_phase, abort, p.status);
+                            // After the first of those: it says that block it - kBufs was drained, so block
+                            // it - kStages before it has landed and `phase` cannot mean the one before that
+                            // (the other warp's block, which this one never waited for).
+                            if (h == 0) ok = ok && bar_wait(&ctl.full[s], phase, abort, p.status);
+                            if (!ok) break;
+                            fence_after();
+#pragma unroll
+                            for (int k = 0; k < kTileK / kMmaK; k++)
+                                mma_f8<PAIR>(tmem + (h * S::kBufs + buf) * 128, da + k * kStepA, db + h * kHalfB + k * kStepB,
+                                             idesc, k > 0);
+                            mma_commit<PAIR>(&ctl.acc[h][buf].full);
+                        }
+                        if (!ok) break;
+                        mma_commit<PAIR>(&ctl.done[s]);
+                        s += 2;
+                        if (s >= S::kStages) s -= S::kStages, phase ^= 1;
+                    }
+                }
+                first = (first + p.blocks_c) & 1;
+                ok = __all_sync(~0u, (int)ok);
+            }
+            if (rank == 0 && !ok && elect_one()) {  // products still in flight end before TMEM is freed
+                mma_commit<PAIR>(&ctl.drain[me]);
+                wait_drain(&ctl.drain[me], 0, kWaitNs);
+            }
+        } else {
+            // ------------------------------------------------ tiles and their scales for the epilogue
+            constexpr int kHalves = BN / 128;
+            uint32_t slot = 0, phase = 1;
+            bool ok = true;
+            while (ok && tiles.next(tile)) {
+                const int row0 = tile.row0 + rank * kTileM;
+                const float *sa[4];
+                const float *sb[kHalves];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int row = row0 + i * 32 + lane;
+                    sa[i] = row < tile.row_end ? p.a_scales + (int64_t)row * p.a_scale_stride : nullptr;
+                }
+#pragma unroll
+                for (int h = 0; h < kHalves; h++) {
+                    // a block of columns wholly past the end has no scale of its own
+                    const int col = tile.col0 + h * 128;
+                    sb[h] = p.w_scales + (int64_t)tile.expert * p.w_scale_expert +
+                            (col < p.out ? (int64_t)(col / 128) * p.w_scale_out : 0);
+                }
+                for (int c0 = 0; c0 < p.blocks_c; c0 += kSlotBlocks) {
+                    const int n = p.blocks_c - c0 < kSlotBlocks ? p.blocks_c - c0 : kSlotBlocks;
+                    float va[kSlotBlocks][4], vb[kSlotBlocks][kHalves];
+#pragma unroll
+                    for (int c = 0; c < kSlotBlocks; c++) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) va[c][i] = c < n && sa[i] ? __ldg(sa[i] + c0 + c) : 0.0f;
+#pragma unroll
+                        for (int h = 0; h < kHalves; h++)
+                            vb[c][h] = c < n ? __ldg(sb[h] + (int64_t)(c0 + c) * p.w_scale_in) : 0.0f;
+                    }
+                    ok = warp_wait(&ctl.slot_empty[slot], phase, abort, p.status);
+                    if (!ok) break;
+                    float *const to = slots + slot * (S::kSlotBytes / 4) + lane;
+#pragma unroll
+                    for (int c = 0; c < kSlotBlocks; c++)
+#pragma unroll
+                        for (int h = 0; h < kHalves; h++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) to[(c * kHalves + h) * 128 + i * 32] = va[c][i] * vb[c][h];
+                    if (lane == 0)
+                        ctl.slot[slot] = make_int4(row0, tile.row_end, tile.col0, n + (c0 + n == p.blocks_c ? kLast : 0));
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&ctl.slot_full[slot]);
+                    if (++slot == kSlots) slot = 0, phase ^= 1;
                 }
             }
-            ok = __shfl_sync(~0u, (int)ok, 0);
-        }
-        if (lane == 0 && !ok)  // copies still in flight land before the CTA ends
-            for (uint32_t k = it > S::kStages ? it - S::kStages : 0; k < it; k++)
-                wait_drain(&ctl.full[k % S::kStages], (k / S::kStages) & 1);
-    } else if (warp == S::kEpiWarps + 1) {
-        // ------------------------------------------------ products
-        constexpr uint32_t idesc = instr_desc(BN, TRANS);
-        uint32_t it = 0;
-        bool ok = true;
-        while (ok && tiles.next(tile, BN)) {
-            if (lane == 0) {
-                for (int c = 0; ok && c < p.blocks_c; c++, it++) {
-                    const uint32_t s = it % S::kStages, buf = it & 1;
-                    if (!bar_wait(&ctl.acc_empty[buf], ((it >> 1) & 1) ^ 1, abort, p.status) ||
-                        !bar_wait(&ctl.full[s], (it / S::kStages) & 1, abort, p.status)) {
-                        ok = false;
-                        break;
-                    }
-                    fence_after();
-                    const uint32_t a = ring + s * S::kStageBytes, b = a + S::kABytes;
-#pragma unroll
-                    for (int k = 0; k < kTileK / kMmaK; k++) {
-                        const uint64_t da = smem_desc(a + k * kMmaK, 16, 1024);
-                        // MN-major: 32 rows of 128 columns further; K-major: 32 bytes along the row
-                        const uint64_t db = TRANS ? smem_desc(b + k * kMmaK * 128, 128 * kTileK, 1024)
-                                                  : smem_desc(b + k * kMmaK, 16, 1024);
-                        mma_f8(tmem + buf * BN, da, db, idesc, k > 0);
-                    }
-                    mma_commit(&ctl.empty[s]);
-                    mma_commit(&ctl.acc_full[buf]);
-                }
+            if (ok && warp_wait(&ctl.slot_empty[slot], phase, abort, p.status) && lane == 0) {  // no more
+                ctl.slot[slot] = make_int4(0, 0, 0, 0);
+                mbar_arrive(&ctl.slot_full[slot]);
             }
-            ok = __shfl_sync(~0u, (int)ok, 0);
-        }
-        if (lane == 0 && !ok) {  // products still in flight end before TMEM is freed
-            mma_commit(&ctl.drain);
-            wait_drain(&ctl.drain, 0);
         }
     } else {
         // ------------------------------------------------ scaling and stores
-        const int lanes0 = (warp & 3) * 32, half = warp >> 2;  // TMEM lanes of this warp; its 128 columns
-        uint32_t it = 0;
-        bool ok = true;
-        while (ok && tiles.next(tile, BN)) {
-            const int64_t row = tile.row0 + lanes0 + lane;
-            const bool mine = row < tile.row_end;
-            const int col0 = tile.col0 + half * 128;
-            const float *sa = p.a_scales + (mine ? row * p.a_scale_stride : 0);
-            // a block of columns wholly past the end has no scale
-            const float *sb = p.w_scales + tile.expert * p.w_scale_expert +
-                              (col0 < p.out ? (int64_t)(col0 / 128) * p.w_scale_out : 0);
-            uint64_t acc[64];
+        // TMEM lanes of this warp, the half it drains, its 64-column groups
+        // there, and where those are in the tile: in a pair, a half's two
+        // groups are 64 columns of either CTA's 128.
+        const int lanes0 = (warp & 3) * 32, half = S::kHalves == 2 ? warp >> 2 : 0, group0 = S::kHalves == 2 ? 0 : warp >> 2;
+        const auto block_of = [&](int u) { return PAIR == 2 ? u : half; };
+        const auto col_of = [&](int u) { return PAIR == 2 ? u * 128 + half * 64 : half * 128 + (group0 + u) * 64; };
+        const uint32_t stage = stages + warp * kPieceBytes;
+        const uint32_t from = tmem + ((uint32_t)lanes0 << 16) + half * S::kBufs * 128 + group0 * 64;
+        const uint32_t empty0 = PAIR == 2 ? in_leader(smem_u32(&ctl.acc[half][0].empty)) : smem_u32(&ctl.acc[half][0].empty);
+        uint32_t slot = 0, phase = 0;
+        uint32_t g = 0;  // blocks so far
+        bool fresh = true;
+        float2 acc[S::kGroups][32];
+        while (warp_wait(&ctl.slot_full[slot], phase, abort, p.status)) {
+            const int4 t = ctl.slot[slot];
+            const int n = t.w & (kLast - 1), row0 = t.x + lanes0;
+            if (n == 0) break;
+            if (fresh) {
 #pragma unroll
-            for (int i = 0; i < 64; i++) acc[i] = 0;
-            float na = mine ? __ldg(sa) : 0.0f, nb = __ldg(sb);
-            for (int c = 0; c < p.blocks_c; c++, it++) {
-                const float s = na * nb;
-                if (c + 1 < p.blocks_c) {  // the next block's scales, ahead of its sums
-                    na = mine ? __ldg(sa + c + 1) : 0.0f;
-                    nb = __ldg(sb + (int64_t)(c + 1) * p.w_scale_in);
-                }
-                const uint32_t buf = it & 1;
-                ok = __all_sync(~0u, bar_wait(&ctl.acc_full[buf], (it >> 1) & 1, abort, p.status));
-                if (!ok) break;  // the whole warp
+                for (int u = 0; u < S::kGroups; u++)
+#pragma unroll
+                    for (int i = 0; i < 32; i++) acc[u][i] = make_float2(0.0f, 0.0f);
+            }
+            const float *scales = slots + slot * (S::kSlotBytes / 4) + lanes0 + lane;
+            bool ok = true;
+#pragma unroll 1
+            for (int c = 0; c < n; c++, g++, scales += BN) {
+                const uint32_t buf = g % S::kBufs;
+                float2 scale[S::kGroups];
+#pragma unroll
+                for (int u = 0; u < S::kGroups; u++) scale[u].x = scale[u].y = scales[block_of(u) * 128];
+                ok = warp_wait(&ctl.acc[half][buf].full, g / S::kBufs & 1, abort, p.status);
+                if (!ok) break;
                 fence_after();
-                const uint32_t from = tmem + ((uint32_t)lanes0 << 16) + buf * BN + half * 128;
-                uint64_t s2;
-                asm("mov.b64 %0, {%1, %1};" : "=l"(s2) : "f"(s));
+                if (row0 < t.y) {  // else no row of this warp is anyone's
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    uint32_t r[32];
-                    tmem_ld32(from + q * 32, r);
-                    tmem_wait_ld(r);
+                    for (int q = 0; q < 4 * S::kGroups; q += S::kAtOnce) {
+                        uint32_t r[S::kAtOnce][16];
 #pragma unroll
-                    for (int i = 0; i < 16; i++) fma2(acc[q * 16 + i], r[2 * i], r[2 * i + 1], s2);
+                        for (int u = 0; u < S::kAtOnce; u++) tmem_ld16(from + buf * 128 + (q + u) * 16, r[u]);
+#pragma unroll
+                        for (int u = 0; u < S::kAtOnce; u++) tmem_wait_ld(r[u]);
+#pragma unroll
+                        for (int u = 0; u < S::kAtOnce; u++)
+#pragma unroll
+                            for (int k = 0; k < 8; k++) {
+                                float2 &a = acc[(q + u) / 4][(q + u) % 4 * 8 + k];
+                                a = __ffma2_rn(make_float2(__uint_as_float(r[u][2 * k]), __uint_as_float(r[u][2 * k + 1])),
+                                               scale[(q + u) / 4], a);
+                            }
+                    }
                 }
                 fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&ctl.acc_empty[buf]);
+                if (lane == 0) arrive_cluster<PAIR>(empty0 + buf * (uint32_t)sizeof(ctl.acc[0][0]));
             }
-            if (ok && mine) {
+            if (!ok) break;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl.slot_empty[slot]);
+            if (++slot == kSlots) slot = 0, phase ^= 1;
+            fresh = t.w & kLast;
+            if (fresh && row0 < t.y) {
 #pragma unroll
-                for (int g = 0; g < 16; g++) {
-                    if (col0 + g * 8 >= p.out) break;
-                    float v[8];
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        asm("mov.b64 {%0, %1}, %2;" : "=f"(v[2 * i]), "=f"(v[2 * i + 1]) : "l"(acc[g * 4 + i]));
-                    store8(p, row, col0 + g * 8, v);
+                for (int u = 0; u < S::kGroups; u++) {
+                    const int col0 = t.z + col_of(u);
+                    if (p.dst_type == SHC_SRC_BF16) store_rows<SHC_SRC_BF16>(p, &map_d, stage, acc[u], row0, t.y, col0);
+                    else if (p.dst_type == SHC_SRC_F16) store_rows<SHC_SRC_F16>(p, &map_d, stage, acc[u], row0, t.y, col0);
+                    else store_rows<SHC_SRC_F32>(p, &map_d, stage, acc[u], row0, t.y, col0);
                 }
             }
         }
+        if (lane == 0) store_wait();
     }
+    __syncwarp();
     fence_before();
-    __syncthreads();
+    sync_all<PAIR>();  // nothing reaches into a CTA that has ended
     fence_after();
-    if (warp == S::kEpiWarps)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::kTmemCols));
+    if (warp == S::kEpiWarps) {
+        if (PAIR == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512));
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512));
+    }
 }
 
 // ---------------------------------------------------------------- host
@@ -471,28 +750,60 @@ bool code_map(CUtensorMap *map, const uint8_t *p, int64_t cols, int64_t rows, in
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int BN, bool TRANS>
-cudaError_t launch(const CUtensorMap &ma, const CUtensorMap &mw, const MmArgs &a, unsigned grid, cudaStream_t st) {
-    using S = Shape<BN>;
+// Rows of D in pieces of 32 rows x 64 bytes.
+bool out_map(CUtensorMap *map, void *p, int64_t cols, int64_t rows, int64_t row_stride, int dst_type) {
+    const int esz = dst_type == SHC_SRC_F32 ? 4 : 2;
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)(row_stride * esz)};
+    const cuuint32_t box[2] = {(cuuint32_t)(64 / esz), 32}, steps[2] = {1, 1};
+    const CUtensorMapDataType t = dst_type == SHC_SRC_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                  : dst_type == SHC_SRC_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                            : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const EncodeTiled f = encode_tiled();
+    return f && f(map, t, 2, p, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+                  CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int BN, int PAIR, bool TRANS>
+cudaError_t launch(const CUtensorMap maps[3], const MmArgs &a, unsigned grid, cudaStream_t st) {
+    using S = Shape<BN, PAIR>;
+    auto *fn = f8_product_kernel<BN, PAIR, TRANS>;
     int per_sm;
-    const cudaError_t e = resident_blocks((const void *)f8_product_kernel<BN, TRANS>, S::kThreads, S::kSmem, &per_sm);
+    const cudaError_t e = resident_blocks((const void *)fn, S::kThreads, S::kSmem, &per_sm);
     if (e != cudaSuccess) return e;
-    f8_product_kernel<BN, TRANS><<<grid, S::kThreads, S::kSmem, st>>>(ma, mw, a);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid * PAIR;
+    cfg.blockDim = S::kThreads;
+    cfg.dynamicSmemBytes = S::kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim = {PAIR, 1, 1};
+    cfg.attrs = &attr;
+    cfg.numAttrs = PAIR > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, fn, maps[0], maps[1], maps[2], a);
+}
+
+template <int BN, int PAIR>
+cudaError_t launch_shape(const CUtensorMap maps[3], const MmArgs &a, bool transposed, int num_sms, cudaStream_t st) {
+    constexpr int TM = kTileM * PAIR;
+    // Tiles there can be at most: every expert with rows may end in a part tile.
+    const int64_t some = a.n_experts < a.n_rows ? a.n_experts : a.n_rows;
+    const int64_t most = (((int64_t)a.n_rows + TM - 1) / TM + (a.offsets ? some : 0)) * ((a.out + BN - 1) / BN);
+    const unsigned grid = (unsigned)(most < num_sms / PAIR ? most : num_sms / PAIR);
+    return transposed ? launch<BN, PAIR, true>(maps, a, grid, st) : launch<BN, PAIR, false>(maps, a, grid, st);
 }
 
 }  // namespace
 
 int launch_f8_product(const F8Product &p, int num_sms, cudaStream_t st) {
-    constexpr int BN = 128;
     const int64_t inner = p.transposed ? p.n : p.k, out = p.transposed ? p.k : p.n;
     MmArgs a{};
     a.a_scales = p.a_scales;
     a.w_scales = p.w_scales;
     a.offsets = p.offsets;
     a.offsets_64 = p.offsets_64;
-    a.n_rows = p.n_rows;
-    a.n_experts = p.n_experts;
+    a.n_rows = (int)p.n_rows;
+    a.n_experts = (int)p.n_experts;
     a.a_scale_stride = p.a_scale_stride;
     const int64_t nb = (p.n + kF8Block - 1) / kF8Block, kb = (p.k + kF8Block - 1) / kF8Block;
     a.w_scale_expert = nb * kb;
@@ -506,17 +817,22 @@ int launch_f8_product(const F8Product &p, int num_sms, cudaStream_t st) {
     const int64_t esz = p.dst_type == SHC_SRC_F32 ? 4 : 2;
     a.vec = ((uintptr_t)p.dst & 15) == 0 && p.dst_row_stride * esz % 16 == 0;
     a.status = p.status;
-    a.a_box = p.n_rows / (p.n_experts > 0 ? p.n_experts : 1) >= kTileM ? kTileM : 32;
+    const int64_t rows_each = p.n_rows / p.n_experts;
+    a.a_box = rows_each >= kTileM ? kTileM : 32;
 
-    CUtensorMap ma, mw;
-    if (!code_map(&ma, p.a, inner, p.n_rows, 1, p.a_row_stride, 0, a.a_box, 2) ||
-        !code_map(&mw, p.w, p.k, p.n, p.n_experts, p.w_row_stride, p.w_mat_stride, 128, 3))
+    CUtensorMap maps[3];
+    if (!code_map(&maps[0], p.a, inner, p.n_rows, 1, p.a_row_stride, 0, a.a_box, 2) ||
+        !code_map(&maps[1], p.w, p.k, p.n, p.n_experts, p.w_row_stride, p.w_mat_stride, 128, 3))
         return SHC_EINVAL;
-    // Tiles there can be at most: every expert with rows may end in a part tile.
-    const int64_t some = p.n_experts < p.n_rows ? p.n_experts : p.n_rows;
-    const int64_t most = ((p.n_rows + kTileM - 1) / kTileM + (p.offsets ? some : 0)) * ((out + BN - 1) / BN);
-    const unsigned grid = (unsigned)(most < num_sms ? most : num_sms);
-    const cudaError_t e = p.transposed ? launch<BN, true>(ma, mw, a, grid, st) : launch<BN, false>(ma, mw, a, grid, st);
+    a.tma_store = a.vec && p.dst_row_stride * esz < ((int64_t)1 << 40) &&
+                  out_map(&maps[2], p.dst, out, p.n_rows, p.dst_row_stride, p.dst_type);
+    if (!a.tma_store) maps[2] = maps[0];
+    // Wide tiles where they fill the machine, in pairs where an expert has rows for several.
+    const int64_t each = (rows_each + kTileM - 1) / kTileM * p.n_experts, wide = each * ((out + 255) / 256);
+    cudaError_t e;
+    if (wide >= num_sms && rows_each >= 1024) e = launch_shape<256, 2>(maps, a, p.transposed, num_sms, st);
+    else if (wide >= num_sms && rows_each >= kTileM) e = launch_shape<256, 1>(maps, a, p.transposed, num_sms, st);
+    else e = launch_shape<128, 1>(maps, a, p.transposed, num_sms, st);
     if (e == cudaSuccess) return SHC_OK;
     return e == cudaErrorMemoryAllocation ? SHC_ENOMEM : SHC_ECUDA;
 }
