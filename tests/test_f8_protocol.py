@@ -61,10 +61,10 @@ def play(rng, stages, bufs, halves, blocks, warps, stage_first=False):
                 while not acc_empty[h][buf].passes(it // bufs & 1 ^ 1):
                     yield
                 assert acc_empty[h][buf].phase == it // bufs
-                if h == 0:
+                if h == 0 and not stage_first:
                     while not full[s].passes(it // stages & 1):
                         yield
-                    assert holds[s] == it
+                assert holds[s] == it
 
                 def finish(h=h, buf=buf, it=it, s=s):
                     assert holds[s] == it
