@@ -39,6 +39,10 @@ constexpr int kMmaK = 32;             // contraction length of one tcgen05 produ
 constexpr int kSlotBlocks = 4;        // contraction blocks whose scales share a slot
 constexpr int kSlots = 3;             // of scales on their way
 constexpr int kPieceBytes = 32 * 64;  // a warp's staging of 32 output rows x 64 bytes
+// Registers: 384 threads start with 168 each, three warps to a scheduler (504
+// of its 512 x 32).  The eight epilogue warps hold up to 128 sums a thread and
+// take 216, the other four keep 72: 2 x 216 + 72 = 504.
+constexpr int kEpiRegs = 216, kOtherRegs = 72;
 constexpr unsigned long long kWaitNs = 4000000000ull;
 constexpr unsigned long long kSettleNs = 2000000ull;
 
@@ -58,7 +62,6 @@ struct Shape {
     static constexpr int kBufs = 512 / BN;
     static_assert(kBufs < kStages, "see the order of the product warps' waits");
     static constexpr int kGroups = BN / 128;  // groups of 64 columns that one epilogue warp drains
-    static constexpr int kAtOnce = BN == 128 ? 4 : 1;  // 16-column TMEM loads in flight, as registers allow
     static constexpr int kSlotBytes = kSlotBlocks * BN * 4;  // [block][BN / 128][128 rows]
     static constexpr size_t kSmem =
         (size_t)kStages * kStageBytes + kEpiWarps * kPieceBytes + kSlots * kSlotBytes + 1024;  // + alignment
@@ -143,7 +146,7 @@ __device__ __forceinline__ bool warp_wait(unsigned long long *b, uint32_t parity
     return __shfl_sync(~0u, ok, 0);
 }
 // After a give-up: wait, bounded, for work that is still in flight.
-__device__ __noinline__ void wait_drain(unsigned long long *b, uint32_t parity, unsigned long long limit_ns) {
+__device__ __forceinline__ void wait_drain(unsigned long long *b, uint32_t parity, unsigned long long limit_ns) {
     const unsigned long long t0 = global_ns();
     while (!bar_test(b, parity) && global_ns() - t0 < limit_ns) {
     }
@@ -481,6 +484,7 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1)
     const uint32_t stages = ring + S::kStages * S::kStageBytes;  // of the epilogue, then the slots of scales
     float *const slots = reinterpret_cast<float *>(smem_raw + (stages - smem_u32(smem_raw)) + S::kEpiWarps * kPieceBytes);
     if (warp >= S::kEpiWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         Tiles<BN, PAIR> tiles(p);
         Tile tile;
         if (warp == S::kEpiWarps) {
@@ -636,6 +640,7 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1)
         }
     } else {
         // ------------------------------------------------ scaling and stores
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
         // TMEM lanes of this warp, the half it drains, its 64-column groups
         // there, and where those are in the tile: in a pair, a half's two
         // groups are 64 columns of either CTA's 128.
@@ -671,21 +676,18 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1)
                 if (!ok) break;
                 fence_after();
                 if (row0 < t.y) {  // else no row of this warp is anyone's
+                    uint32_t r[2][16];
+                    tmem_ld16(from + buf * 128, r[0]);
 #pragma unroll
-                    for (int q = 0; q < 4 * S::kGroups; q += S::kAtOnce) {
-                        uint32_t r[S::kAtOnce][16];
+                    for (int q = 0; q < 4 * S::kGroups; q++) {
+                        tmem_wait_ld(r[q & 1]);
+                        if (q + 1 < 4 * S::kGroups) tmem_ld16(from + buf * 128 + (q + 1) * 16, r[(q + 1) & 1]);
 #pragma unroll
-                        for (int u = 0; u < S::kAtOnce; u++) tmem_ld16(from + buf * 128 + (q + u) * 16, r[u]);
-#pragma unroll
-                        for (int u = 0; u < S::kAtOnce; u++) tmem_wait_ld(r[u]);
-#pragma unroll
-                        for (int u = 0; u < S::kAtOnce; u++)
-#pragma unroll
-                            for (int k = 0; k < 8; k++) {
-                                float2 &a = acc[(q + u) / 4][(q + u) % 4 * 8 + k];
-                                a = __ffma2_rn(make_float2(__uint_as_float(r[u][2 * k]), __uint_as_float(r[u][2 * k + 1])),
-                                               scale[(q + u) / 4], a);
-                            }
+                        for (int k = 0; k < 8; k++) {
+                            float2 &a = acc[q / 4][q % 4 * 8 + k];
+                            a = __ffma2_rn(make_float2(__uint_as_float(r[q & 1][2 * k]), __uint_as_float(r[q & 1][2 * k + 1])),
+                                           scale[q / 4], a);
+                        }
                     }
                 }
                 fence_before();
