@@ -6,6 +6,7 @@ come from PyTorch; every byte of encoding, decoding and error measurement is
 computed by the CUDA kernels in shoehorn_b200/csrc.  There is no CPU fallback:
 if the library or a CUDA device is missing, the calls raise.
 """
+import contextlib
 import ctypes
 import enum
 import os
@@ -149,6 +150,9 @@ def grid_info(which):
     return gs.value, kmap, nb
 
 
+_HERE_AND_NOW = contextlib.nullcontext()
+
+
 class Context:
     """A library context bound to one CUDA device (shc_init/shc_free)."""
 
@@ -273,23 +277,21 @@ class Context:
     # Single-token calls are bound by the host, so each tensor's size, strides
     # and device are asked for once.
 
-    def _f8_on(self, stream, fresh, *tensors):
-        """Allocates results (`fresh`) on the stream the work goes to, and
-        keeps the tensors' memory until that work is done where it is not the
-        current one.  Returns (results, stream handle)."""
+    def _f8_on(self, stream, *tensors):
+        """(handle of the stream the work goes to, the context to allocate
+        its results in).  Where that is not the current stream, the tensors'
+        memory is kept until the work is done."""
         torch = self.torch
         if stream is None:
-            return fresh(), self._f8_stream()
+            return self._f8_stream(), _HERE_AND_NOW
         if stream.device.index != self.device:
             raise ValueError(f"stream of cuda:{stream.device.index} in a context of cuda:{self.device}")
         if stream == torch.cuda.current_stream(self.device):
-            return fresh(), stream.cuda_stream
-        with torch.cuda.stream(stream):
-            made = fresh()
+            return stream.cuda_stream, _HERE_AND_NOW
         for t in tensors:
             if t is not None:
                 t.record_stream(stream)
-        return made, stream.cuda_stream
+        return stream.cuda_stream, torch.cuda.stream(stream)
 
     def _f8_stream(self):
         raw = getattr(self.torch._C, "_cuda_getCurrentRawStream", None)
@@ -386,17 +388,15 @@ class Context:
         pitch = (cols + 15) // 16 * 16
         step = rows * pitch
 
-        def fresh():
-            o, s = out, scales
-            if o is None:
-                o = torch.empty((*lead, rows, pitch), dtype=torch.float8_e4m3fn, device=src.device)
+        stp, on = self._f8_on(stream, src, out, scales)
+        with on:
+            codes, made = out, scales
+            if codes is None:
+                codes = src.new_empty((*lead, rows, pitch), dtype=torch.float8_e4m3fn)
                 if pitch != cols:
-                    o = o[..., :cols]
-            if s is None:
-                s = torch.empty(blocks, dtype=torch.float32, device=src.device)
-            return o, s
-
-        (codes, made), stp = self._f8_on(stream, fresh, src, out, scales)
+                    codes = codes[..., :cols]
+            if made is None:
+                made = src.new_empty(blocks, dtype=torch.float32)
         if out is not None:
             pitch, step = self._f8_codes(out, "out", (2, 3))[3:]
         if scales is not None:
@@ -426,10 +426,9 @@ class Context:
             if out.dtype is not dtype or out.shape != shape or not out.is_contiguous():
                 raise ValueError("out must be contiguous, of codes' shape and of dtype")
 
-        def fresh():
-            return torch.empty(shape, dtype=dtype, device=codes.device) if out is None else out
-
-        res, stp = self._f8_on(stream, fresh, codes, scales, out)
+        stp, on = self._f8_on(stream, codes, scales, out)
+        with on:
+            res = codes.new_empty(shape, dtype=dtype) if out is None else out
         rc = lib().shc_decode_f8(self.handle, dt, codes.data_ptr(), mats, rows, cols, pitch, step, block_rows,
                                  scales.data_ptr(), res.data_ptr(), stp)
         if rc:
@@ -461,10 +460,9 @@ class Context:
             if (cols > 1 and out.stride(1) != 1) or pitch_o < cols:
                 raise ValueError("out's columns must be adjacent and its rows apart")
 
-        def fresh():
-            return torch.empty((rows, cols), dtype=dtype, device=a.device) if out is None else out
-
-        res, stp = self._f8_on(stream, fresh, a, a_scales, w, w_scales, offsets, out)
+        stp, on = self._f8_on(stream, a, a_scales, w, w_scales, offsets, out)
+        with on:
+            res = a.new_empty((rows, cols), dtype=dtype) if out is None else out
         if offsets is None:
             rc = lib().shc_matmul_f8(self.handle, a.data_ptr(), pitch_a, a_scales.data_ptr(), pitch_s, rows, w.data_ptr(),
                                      pitch_w, w_scales.data_ptr(), n, k, transposed, dt, res.data_ptr(), pitch_o, stp)

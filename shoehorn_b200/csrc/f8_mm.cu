@@ -78,10 +78,11 @@ struct MmArgs {
     int out;       // output columns
     int blocks_c;  // contraction blocks
     int a_box;     // rows of one box of A
+    int split;     // CTAs (a cluster of them) that share a tile's contraction
     void *dst;
     int64_t dst_row_stride;
     int dst_type;
-    int vec;        // rows of dst start on 16-byte boundaries
+    int align;      // bytes that every row of dst starts on a multiple of: 16, 8 or fewer
     int tma_store;  // map_d describes dst
     int *status;
 };
@@ -95,6 +96,7 @@ struct Control {
     unsigned long long slot_full[kSlots], slot_empty[kSlots];
     unsigned long long drain[2];
     int4 slot[kSlots];  // what a slot's scales are for: first row of this CTA, end of rows, first column, blocks (see kLast)
+    int4 joined;  // SPLIT: first row, rows and first column of the tile whose sums are in the ring
     uint32_t tmem;
     int abort;
 };
@@ -155,6 +157,10 @@ __device__ __forceinline__ void expect_tx(unsigned long long *b, uint32_t bytes)
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(b)), "r"(bytes) : "memory");
 }
 
+__device__ __forceinline__ void st_shared(uint32_t addr, float v) {
+    asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+
 // ---------------------------------------------------------------- TMA, tcgen05
 
 // Loads signal `bar`, an address in the cluster's shared window: the CTA's
@@ -195,6 +201,16 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, uint32_t sr
 __device__ __forceinline__ void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
+// f32 at a shared address of another CTA of the cluster.
+__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
+    float v;
+    asm volatile(
+        "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %1, %2;\n ld.shared::cluster.f32 %0, [a];\n}"
+        : "=f"(v)
+        : "r"(addr), "r"(rank)
+        : "memory");
+    return v;
+}
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -215,9 +231,9 @@ __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
     if (PAIR == 2) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
     else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-template <int PAIR>
+template <bool CLUSTER>
 __device__ __forceinline__ void sync_all() {
-    if (PAIR == 2) {
+    if (CLUSTER) {
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     } else {
@@ -305,7 +321,7 @@ struct Tiles {
     int64_t t, base;  // base: tiles before expert e0
     int e0;
     const MmArgs &p;
-    __device__ __forceinline__ Tiles(const MmArgs &args) : t(blockIdx.x / PAIR), base(0), e0(0), p(args) {}
+    __device__ __forceinline__ Tiles(const MmArgs &args) : t(blockIdx.x / (PAIR * args.split)), base(0), e0(0), p(args) {}
     __device__ __forceinline__ int offset(int e) const {
         const int64_t v = p.offsets_64 ? static_cast<const int64_t *>(p.offsets)[e]
                                        : (int64_t) static_cast<const int32_t *>(p.offsets)[e];
@@ -340,7 +356,7 @@ struct Tiles {
                 o.col0 = (int)ct * BN;
                 o.row0 = lo + (int)(at - ct * mt) * TM;
                 o.row_end = hi;
-                t += gridDim.x / PAIR;
+                t += gridDim.x / (PAIR * p.split);
                 return true;
             }
             base += __shfl_sync(~0u, sum, 31);
@@ -402,13 +418,24 @@ __device__ __forceinline__ void store_rows(const MmArgs &p, const CUtensorMap *m
         const int rows = row_end - row0 < 32 ? row_end - row0 : 32;
         uint8_t *d = static_cast<uint8_t *>(p.dst) + ((int64_t)row0 * p.dst_row_stride + col) * esz;
         const int64_t pitch = p.dst_row_stride * esz;
-        if (p.vec && col + kCols <= p.out) {
+        // Rows of the piece: 16 bytes a lane where rows of D start on 16-byte
+        // boundaries, 8 where they start on 8-byte ones, else single elements.
+        if (p.align >= 16 && col + kCols <= p.out) {
             for (int r = lane >> 2; r < rows; r += 8) {
                 uint32_t w[4];
                 asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                              : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
                              : "r"(stage + r * 64 + (((lane & 3) ^ (r >> 1 & 3)) << 4)));
                 *reinterpret_cast<uint4 *>(d + r * pitch + (lane & 3) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        } else if (p.align == 8 && col + kCols <= p.out) {
+            const int k = lane & 7;
+            for (int r = lane >> 3; r < rows; r += 4) {
+                uint32_t w[2];
+                asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
+                             : "=r"(w[0]), "=r"(w[1])
+                             : "r"(stage + r * 64 + (((k >> 1) ^ (r >> 1 & 3)) << 4) + (k & 1) * 8));
+                *reinterpret_cast<uint2 *>(d + r * pitch + k * 8) = make_uint2(w[0], w[1]);
             }
         } else {
             // kCols columns of 32 / kCols rows at once
@@ -434,7 +461,38 @@ __device__ __forceinline__ void store_rows(const MmArgs &p, const CUtensorMap *m
 
 // ---------------------------------------------------------------- kernel
 
-template <int BN, int PAIR, bool TRANS>
+// Four columns of one row of D, for the joined parts of a split tile.
+__device__ __forceinline__ void store4(const MmArgs &p, int row, int col, const float v[4]) {
+    const int64_t at = (int64_t)row * p.dst_row_stride + col;
+    const bool whole = p.align >= 16 && col + 4 <= p.out;
+    if (p.dst_type == SHC_SRC_F32) {
+        float *d = static_cast<float *>(p.dst) + at;
+        if (whole) {
+            *reinterpret_cast<float4 *>(d) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (col + i < p.out) d[i] = v[i];
+        }
+        return;
+    }
+    uint16_t *d = static_cast<uint16_t *>(p.dst) + at;
+    const float2 lo = make_float2(v[0], v[1]), hi = make_float2(v[2], v[3]);
+    const uint2 w = p.dst_type == SHC_SRC_F16 ? make_uint2(pack_f16(lo), pack_f16(hi)) : make_uint2(pack_bf16(lo), pack_bf16(hi));
+    if (whole) {
+        *reinterpret_cast<uint2 *>(d) = w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (col + i < p.out) d[i] = (uint16_t)((i < 2 ? w.x : w.y) >> (16 * (i & 1)));
+    }
+}
+
+// SPLIT (with BN = 128, PAIR = 1): a cluster of p.split CTAs shares one tile,
+// each taking an equal run of its contraction blocks.  They leave their sums
+// in their rings, which nothing else uses by then, and each adds up (always
+// in rank order) and stores its share of the columns.
+template <int BN, int PAIR, bool TRANS, bool SPLIT>
 __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1)
     f8_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
                       const __grid_constant__ CUtensorMap map_d, const __grid_constant__ MmArgs p) {
@@ -444,6 +502,9 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1)
     const uint32_t ring = (smem_u32(smem_raw) + 1023) & ~1023u;  // the swizzle's pattern repeats every 1024 bytes
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     const int rank = PAIR == 2 ? (int)cluster_rank() : 0;
+    const int part = SPLIT ? (int)cluster_rank() : 0;
+    const int c_begin = SPLIT ? p.blocks_c * part / p.split : 0;  // this CTA's contraction blocks
+    const int blocks = SPLIT ? p.blocks_c * (part + 1) / p.split - c_begin : p.blocks_c;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; s++) {
@@ -461,6 +522,7 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1)
         }
         for (int i = 0; i < 2; i++) mbar_init(&ctl.drain[i], 1);
         ctl.abort = 0;
+        ctl.joined = make_int4(0, 0, 0, 0);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == S::kEpiWarps) {
@@ -476,7 +538,7 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1)
     }
     fence_before();
     __syncthreads();
-    if (PAIR == 2) sync_all<PAIR>();  // both CTAs' barriers are set up
+    if (PAIR == 2) sync_all<true>();  // both CTAs' barriers are set up
     fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&ctl.tmem);
     volatile int *abort = &ctl.abort;
@@ -504,7 +566,7 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1)
 #pragma unroll
                 for (int r = 0; r < PAIR; r++) bytes += boxes[r] * p.a_box * kTileK + S::kBBytes;
                 if (elect_one()) {
-                    for (int c = 0; c < p.blocks_c; c++) {
+                    for (int c = c_begin; c < c_begin + blocks; c++) {
                         const uint32_t s = it % S::kStages, round = it / S::kStages;
                         if (!bar_wait(&ctl.done[s], (round & 1) ^ 1, abort, p.status)) {
                             ok = false;
@@ -554,7 +616,7 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1)
             bool ok = rank == 0;
             while (ok && tiles.next(tile)) {
                 if (elect_one()) {
-                    for (uint32_t c = first; c < (uint32_t)p.blocks_c; c += 2, it += 2) {
+                    for (uint32_t c = first; c < (uint32_t)blocks; c += 2, it += 2) {
                         const uint32_t buf = it % S::kBufs, acc_phase = ((it / S::kBufs) & 1) ^ 1;
                         const uint64_t da = da0 + (uint64_t)(s * (S::kStageBytes >> 4)), db = db0 + (uint64_t)(s * (S::kStageBytes >> 4));
 #pragma unroll
@@ -578,7 +640,7 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1)
                         if (s >= S::kStages) s -= S::kStages, phase ^= 1;
                     }
                 }
-                first = (first + p.blocks_c) & 1;
+                first = (first + blocks) & 1;
                 ok = __all_sync(~0u, (int)ok);
             }
             if (rank == 0 && !ok && elect_one()) {  // products still in flight end before TMEM is freed
@@ -606,16 +668,16 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1)
                     sb[h] = p.w_scales + (int64_t)tile.expert * p.w_scale_expert +
                             (col < p.out ? (int64_t)(col / 128) * p.w_scale_out : 0);
                 }
-                for (int c0 = 0; c0 < p.blocks_c; c0 += kSlotBlocks) {
-                    const int n = p.blocks_c - c0 < kSlotBlocks ? p.blocks_c - c0 : kSlotBlocks;
+                for (int c0 = 0; c0 < blocks; c0 += kSlotBlocks) {
+                    const int n = blocks - c0 < kSlotBlocks ? blocks - c0 : kSlotBlocks;
                     float va[kSlotBlocks][4], vb[kSlotBlocks][kHalves];
 #pragma unroll
                     for (int c = 0; c < kSlotBlocks; c++) {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) va[c][i] = c < n && sa[i] ? __ldg(sa[i] + c0 + c) : 0.0f;
+                        for (int i = 0; i < 4; i++) va[c][i] = c < n && sa[i] ? __ldg(sa[i] + c_begin + c0 + c) : 0.0f;
 #pragma unroll
                         for (int h = 0; h < kHalves; h++)
-                            vb[c][h] = c < n ? __ldg(sb[h] + (int64_t)(c0 + c) * p.w_scale_in) : 0.0f;
+                            vb[c][h] = c < n ? __ldg(sb[h] + (int64_t)(c_begin + c0 + c) * p.w_scale_in) : 0.0f;
                     }
                     ok = warp_wait(&ctl.slot_empty[slot], phase, abort, p.status);
                     if (!ok) break;
@@ -627,7 +689,7 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1)
 #pragma unroll
                             for (int i = 0; i < 4; i++) to[(c * kHalves + h) * 128 + i * 32] = va[c][i] * vb[c][h];
                     if (lane == 0)
-                        ctl.slot[slot] = make_int4(row0, tile.row_end, tile.col0, n + (c0 + n == p.blocks_c ? kLast : 0));
+                        ctl.slot[slot] = make_int4(row0, tile.row_end, tile.col0, n + (c0 + n == blocks ? kLast : 0));
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&ctl.slot_full[slot]);
                     if (++slot == kSlots) slot = 0, phase ^= 1;
@@ -699,7 +761,17 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1)
             if (lane == 0) mbar_arrive(&ctl.slot_empty[slot]);
             if (++slot == kSlots) slot = 0, phase ^= 1;
             fresh = t.w & kLast;
-            if (fresh && row0 < t.y) {
+            if (SPLIT && fresh) {
+                if (threadIdx.x == 0) ctl.joined = make_int4(t.x, t.y - t.x < kTileM ? t.y - t.x : kTileM, t.z, 0);
+                if (row0 < t.y) {
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        const uint32_t at = ring + ((group0 * 64 + 2 * i) * kTileM + lanes0 + lane) * 4;
+                        st_shared(at, acc[0][i].x);
+                        st_shared(at + kTileM * 4, acc[0][i].y);
+                    }
+                }
+            } else if (fresh && row0 < t.y) {
 #pragma unroll
                 for (int u = 0; u < S::kGroups; u++) {
                     const int col0 = t.z + col_of(u);
@@ -712,8 +784,29 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1)
         if (lane == 0) store_wait();
     }
     __syncwarp();
+    if (SPLIT) {
+        sync_all<true>();  // every part's sums are in its ring
+        const int4 joined = ctl.joined;
+        // Items of one row x four columns; all parts' sums of an item are on their way at once.
+        const int wide = kTileM / p.split;  // columns of this CTA
+        for (int at = threadIdx.x; at < joined.y * (wide / 4); at += S::kThreads) {
+            const int c = at / joined.y, row = at - c * joined.y, col = part * wide + c * 4;
+            float v[8][4];
+#pragma unroll
+            for (int q = 0; q < 8; q++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    v[q][i] = q < p.split ? ld_cluster(ring + ((col + i) * kTileM + row) * 4, q) : 0.0f;
+#pragma unroll
+            for (int q = 1; q < 8; q++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[0][i] += v[q][i];
+            store4(p, joined.x + row, joined.z + col, v[0]);
+        }
+        __syncwarp();
+    }
     fence_before();
-    sync_all<PAIR>();  // nothing reaches into a CTA that has ended
+    sync_all<PAIR == 2 || SPLIT>();  // nothing reaches into a CTA that has ended
     fence_after();
     if (warp == S::kEpiWarps) {
         if (PAIR == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512));
@@ -765,34 +858,54 @@ bool out_map(CUtensorMap *map, void *p, int64_t cols, int64_t rows, int64_t row_
                   CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int BN, int PAIR, bool TRANS>
+template <int BN, int PAIR, bool TRANS, bool SPLIT>
 cudaError_t launch(const CUtensorMap maps[3], const MmArgs &a, unsigned grid, cudaStream_t st) {
     using S = Shape<BN, PAIR>;
-    auto *fn = f8_product_kernel<BN, PAIR, TRANS>;
+    auto *fn = f8_product_kernel<BN, PAIR, TRANS, SPLIT>;
     int per_sm;
     const cudaError_t e = resident_blocks((const void *)fn, S::kThreads, S::kSmem, &per_sm);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid * PAIR;
+    cfg.gridDim = grid * PAIR * a.split;
     cfg.blockDim = S::kThreads;
     cfg.dynamicSmemBytes = S::kSmem;
     cfg.stream = st;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim = {PAIR, 1, 1};
+    attr.val.clusterDim = {(unsigned)(PAIR * a.split), 1, 1};
     cfg.attrs = &attr;
-    cfg.numAttrs = PAIR > 1 ? 1 : 0;
+    cfg.numAttrs = PAIR * a.split > 1 ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, fn, maps[0], maps[1], maps[2], a);
 }
 
-template <int BN, int PAIR>
-cudaError_t launch_shape(const CUtensorMap maps[3], const MmArgs &a, bool transposed, int num_sms, cudaStream_t st) {
-    constexpr int TM = kTileM * PAIR;
-    // Tiles there can be at most: every expert with rows may end in a part tile.
+// Tiles there can be at most: every expert with rows may end in a part tile.
+int64_t most_tiles(const MmArgs &a, int tm, int bn) {
     const int64_t some = a.n_experts < a.n_rows ? a.n_experts : a.n_rows;
-    const int64_t most = (((int64_t)a.n_rows + TM - 1) / TM + (a.offsets ? some : 0)) * ((a.out + BN - 1) / BN);
+    return (((int64_t)a.n_rows + tm - 1) / tm + (a.offsets ? some : 0)) * ((a.out + bn - 1) / bn);
+}
+
+// CTAs to share a tile's contraction where the tiles alone leave most SMs
+// idle.  Measured (1 to 256 rows, 1024 to 4096 columns, 8 to 112 blocks): a
+// block takes 0.28 us, joining two parts 1.7 us + 3.5 us x rows / 128 and
+// four or eight 1.3 + 2.8 x rows / 128, whatever the number of blocks.  So one
+// row through 4096 x 4096 takes 8.7 us in four parts (13.4 in one), 128 rows
+// through 2048 x 1024 8.1 (6.1 in one: not split).  Clusters of eight do not
+// all run at once beyond 64 CTAs (16 of them take twice as long as 8).
+int split_for(int64_t tiles, int blocks, int rows, int num_sms) {
+    int best = 1, least = 28 * blocks;
+    for (int z = 2; z <= 8; z *= 2) {
+        if (tiles * z > (z == 8 ? 64 : num_sms) || blocks < 2 * z) break;
+        const int time = 28 * blocks / z + (z == 2 ? 170 + 350 * rows / 128 : 130 + 280 * rows / 128);
+        if (time < least) least = time, best = z;
+    }
+    return best;
+}
+
+template <int BN, int PAIR, bool SPLIT = false>
+cudaError_t launch_shape(const CUtensorMap maps[3], const MmArgs &a, bool transposed, int num_sms, cudaStream_t st) {
+    const int64_t most = most_tiles(a, kTileM * PAIR, BN);
     const unsigned grid = (unsigned)(most < num_sms / PAIR ? most : num_sms / PAIR);
-    return transposed ? launch<BN, PAIR, true>(maps, a, grid, st) : launch<BN, PAIR, false>(maps, a, grid, st);
+    return transposed ? launch<BN, PAIR, true, SPLIT>(maps, a, grid, st) : launch<BN, PAIR, false, SPLIT>(maps, a, grid, st);
 }
 
 }  // namespace
@@ -817,7 +930,8 @@ int launch_f8_product(const F8Product &p, int num_sms, cudaStream_t st) {
     a.dst_row_stride = p.dst_row_stride;
     a.dst_type = p.dst_type;
     const int64_t esz = p.dst_type == SHC_SRC_F32 ? 4 : 2;
-    a.vec = ((uintptr_t)p.dst & 15) == 0 && p.dst_row_stride * esz % 16 == 0;
+    const uint64_t starts = (uintptr_t)p.dst | (uint64_t)(p.dst_row_stride * esz);
+    a.align = starts % 16 == 0 ? 16 : starts % 8 == 0 ? 8 : 1;
     a.status = p.status;
     const int64_t rows_each = p.n_rows / p.n_experts;
     a.a_box = rows_each >= kTileM ? kTileM : 32;
@@ -826,13 +940,15 @@ int launch_f8_product(const F8Product &p, int num_sms, cudaStream_t st) {
     if (!code_map(&maps[0], p.a, inner, p.n_rows, 1, p.a_row_stride, 0, a.a_box, 2) ||
         !code_map(&maps[1], p.w, p.k, p.n, p.n_experts, p.w_row_stride, p.w_mat_stride, 128, 3))
         return SHC_EINVAL;
-    a.tma_store = a.vec && p.dst_row_stride * esz < ((int64_t)1 << 40) &&
+    a.tma_store = a.align == 16 && p.dst_row_stride * esz < ((int64_t)1 << 40) &&
                   out_map(&maps[2], p.dst, out, p.n_rows, p.dst_row_stride, p.dst_type);
     if (!a.tma_store) maps[2] = maps[0];
     // Wide tiles where they fill the machine, in pairs where an expert has rows for several.
     const int64_t each = (rows_each + kTileM - 1) / kTileM * p.n_experts, wide = each * ((out + 255) / 256);
     cudaError_t e;
-    if (wide >= num_sms && rows_each >= 1024) e = launch_shape<256, 2>(maps, a, p.transposed, num_sms, st);
+    a.split = split_for(most_tiles(a, kTileM, 128), a.blocks_c, (int)(rows_each < kTileM ? rows_each : kTileM), num_sms);
+    if (a.split > 1) e = launch_shape<128, 1, true>(maps, a, p.transposed, num_sms, st);
+    else if (wide >= num_sms && rows_each >= 1024) e = launch_shape<256, 2>(maps, a, p.transposed, num_sms, st);
     else if (wide >= num_sms && rows_each >= kTileM) e = launch_shape<256, 1>(maps, a, p.transposed, num_sms, st);
     else e = launch_shape<128, 1>(maps, a, p.transposed, num_sms, st);
     if (e == cudaSuccess) return SHC_OK;
