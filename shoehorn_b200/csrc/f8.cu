@@ -40,18 +40,43 @@ struct Raw {
     static constexpr int kWords = ST == SHC_SRC_F32 ? 16 : 8;
     uint32_t w[kWords];
 
-    // Columns col.. of the row at p (on a 16-byte boundary), zeros from ne0 on.
-    __device__ __forceinline__ void load(const uint8_t *p, int64_t col, int64_t ne0) {
+    // Columns col.. of the row at p, zeros from ne0 on.  VEC: the row starts
+    // on a 16-byte boundary.  Otherwise the aligned 16-byte words around the
+    // columns are loaded and shifted into place (elements one by one took 3
+    // times as long), as long as they lie within [lo, hi), the source's bytes.
+    template <bool VEC>
+    __device__ __forceinline__ void load(const uint8_t *p, int64_t col, int64_t ne0, const uint8_t *lo, const uint8_t *hi) {
         constexpr int esz = ST == SHC_SRC_F32 ? 4 : 2;
-        if (col + kElems <= ne0) {
-            const uint4 *q = reinterpret_cast<const uint4 *>(p + col * esz);
+        const uint8_t *from = p + col * esz;
+        const int off = VEC ? 0 : (int)((uintptr_t)from & 15);
+        if (col >= ne0) {
+            zero();
+        } else if (VEC ? col + kElems <= ne0 : from - off >= lo && from - off + 4 * kWords + 16 <= hi) {
+            const uint4 *q = reinterpret_cast<const uint4 *>(from - off);
+            uint32_t x[kWords + 4];
 #pragma unroll
-            for (int i = 0; i < kWords / 4; i++) {
-                const uint4 v = __ldcs(q + i);  // read once
-                w[4 * i] = v.x;
-                w[4 * i + 1] = v.y;
-                w[4 * i + 2] = v.z;
-                w[4 * i + 3] = v.w;
+            for (int i = 0; i < kWords / 4 + (VEC ? 0 : 1); i++) {
+                const uint4 v = VEC ? __ldcs(q + i) : __ldg(q + i);  // aligned words are read once, others by two lanes
+                x[4 * i] = v.x;
+                x[4 * i + 1] = v.y;
+                x[4 * i + 2] = v.z;
+                x[4 * i + 3] = v.w;
+            }
+            if (!VEC) {
+#pragma unroll
+                for (int i = 0; i < kWords + 2; i++) x[i] = off & 8 ? x[i + 2] : x[i];
+#pragma unroll
+                for (int i = 0; i < kWords + 1; i++) x[i] = off & 4 ? x[i + 1] : x[i];
+            }
+#pragma unroll
+            for (int i = 0; i < kWords; i++) w[i] = !VEC && esz == 2 && off & 2 ? __funnelshift_r(x[i], x[i + 1], 16) : x[i];
+            if (!VEC && col + kElems > ne0) {
+                const int n = (int)(ne0 - col);
+#pragma unroll
+                for (int i = 0; i < kWords; i++) {
+                    if (esz == 4) w[i] = i < n ? w[i] : 0u;
+                    else w[i] = 2 * i + 1 < n ? w[i] : 2 * i < n ? w[i] & 0xFFFFu : 0u;
+                }
             }
         } else if (ST == SHC_SRC_F32) {
 #pragma unroll
@@ -61,9 +86,9 @@ struct Raw {
             const uint16_t *q = reinterpret_cast<const uint16_t *>(p) + col;
 #pragma unroll
             for (int i = 0; i < kWords; i++) {
-                const uint32_t lo = col + 2 * i < ne0 ? __ldg(q + 2 * i) : 0u;
-                const uint32_t hi = col + 2 * i + 1 < ne0 ? __ldg(q + 2 * i + 1) : 0u;
-                w[i] = lo | hi << 16;
+                const uint32_t a = col + 2 * i < ne0 ? __ldg(q + 2 * i) : 0u;
+                const uint32_t b = col + 2 * i + 1 < ne0 ? __ldg(q + 2 * i + 1) : 0u;
+                w[i] = a | b << 16;
             }
         }
     }
@@ -133,6 +158,11 @@ __device__ __forceinline__ const uint8_t *src_row(const F8Codec &c, int64_t mat,
     return static_cast<const uint8_t *>(c.src) + (mat * c.src_mat_stride + r * c.src_row_stride) * (ST == SHC_SRC_F32 ? 4 : 2);
 }
 
+template <int ST>
+__device__ __forceinline__ const uint8_t *src_end(const F8Codec &c) {
+    return src_row<ST>(c, c.n_mats - 1, c.n_rows - 1) + c.ne0 * (ST == SHC_SRC_F32 ? 4 : 2);
+}
+
 // Activations: eight lanes per (row, block), kUnits of them at once so that a
 // warp has kUnits x 4 blocks' loads in flight.  I: unit index type, 32 bits
 // wherever the units can be counted in them (a division by the row's blocks
@@ -140,12 +170,13 @@ __device__ __forceinline__ const uint8_t *src_row(const F8Codec &c, int64_t mat,
 template <int ST>
 __host__ __device__ constexpr int units() { return ST == SHC_SRC_F32 ? 2 : 4; }
 
-template <int ST, typename I>
+template <int ST, bool VEC, typename I>
 __global__ void __launch_bounds__(256) f8_encode_rows_kernel(F8Codec c) {
     constexpr int kUnits = units<ST>(), kPerBlock = 256 / kLanes;
     const I nb = (I)((c.ne0 + kF8Block - 1) / kF8Block), total = (I)(c.n_mats * c.n_rows) * nb, rows = (I)c.n_rows;
     const int lane = threadIdx.x & (kLanes - 1);
     const I u0 = (I)blockIdx.x * (kPerBlock * kUnits) + threadIdx.x / kLanes;
+    const uint8_t *const lo = src_row<ST>(c, 0, 0), *const hi = src_end<ST>(c);
     Raw<ST> v[kUnits];
     uint8_t *row[kUnits];
     int64_t col[kUnits];
@@ -158,7 +189,7 @@ __global__ void __launch_bounds__(256) f8_encode_rows_kernel(F8Codec c) {
         col[k] = (int64_t)b * kF8Block + lane * kElems;
         if (u >= total) col[k] = c.ne0;
         row[k] = c.codes + (int64_t)mat * c.code_mat_stride + (int64_t)r * c.code_row_stride;
-        v[k].load(src_row<ST>(c, mat, r), col[k], c.ne0);
+        v[k].template load<VEC>(src_row<ST>(c, mat, r), col[k], c.ne0, lo, hi);
     }
     bool inf = false;
 #pragma unroll
@@ -187,19 +218,20 @@ __global__ void __launch_bounds__(256) f8_encode_rows_kernel(F8Codec c) {
 
 // Weights: one thread block per 128 x 128 tile, held in registers between the
 // maximum and the codes; thread t has 16 columns of rows t / 8 + 32 i.
-template <int ST>
+template <int ST, bool VEC>
 __global__ void __launch_bounds__(256) f8_encode_tiles_kernel(F8Codec c) {
     const int64_t nb = (c.ne0 + kF8Block - 1) / kF8Block, rb = (c.n_rows + kF8Block - 1) / kF8Block;
     const int64_t tile = blockIdx.x, b = tile % nb, rest = tile / nb, mat = rest / rb;
     const int64_t row0 = (rest - mat * rb) * kF8Block + threadIdx.x / kLanes;
     const int64_t col = b * kF8Block + (threadIdx.x & (kLanes - 1)) * kElems;
     __shared__ float s_top[2][8];
+    const uint8_t *const lo = src_row<ST>(c, 0, 0), *const hi = src_end<ST>(c);
     Raw<ST> v[4];
     float m = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int64_t r = row0 + 32 * i;
-        if (r < c.n_rows) v[i].load(src_row<ST>(c, mat, r), col, c.ne0);
+        if (r < c.n_rows) v[i].template load<VEC>(src_row<ST>(c, mat, r), col, c.ne0, lo, hi);
         else v[i].zero();
     }
 #pragma unroll
@@ -227,117 +259,6 @@ __global__ void __launch_bounds__(256) f8_encode_tiles_kernel(F8Codec c) {
     if (threadIdx.x == 0) c.scales[tile] = m / kF8Top;
 }
 
-// Rows that start at any element: a warp per (row, block), lane l on columns l,
-// l + 32, l + 64 and l + 96, so that loads and code bytes of a warp are
-// adjacent whatever the alignment (16 columns a lane as above took 4 times as
-// long: 8192 x 14330 bf16 250 us).
-template <int ST>
-__device__ __forceinline__ float load_any(const uint8_t *row, int64_t col) {
-    if (ST == SHC_SRC_F32) return __ldg(reinterpret_cast<const float *>(row) + col);
-    const uint16_t h = __ldg(reinterpret_cast<const uint16_t *>(row) + col);
-    return ST == SHC_SRC_BF16 ? bf16_bits_to_f32(h) : f16_val(h);
-}
-// The block's largest finite magnitude over a warp's v; infinite elements become NaN.
-template <int N>
-__device__ __forceinline__ float warp_top(float v[N], bool &inf) {
-    float m = 0.0f;
-#pragma unroll
-    for (int j = 0; j < N; j++) m = fmaxf(m, fabsf(v[j]));
-#pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-    inf = m == inf_f();
-    return m;
-}
-template <int N>
-__device__ __forceinline__ float warp_top_finite(float v[N]) {
-    float m = 0.0f;
-#pragma unroll
-    for (int j = 0; j < N; j++) {
-        if (fabsf(v[j]) == inf_f()) v[j] = __uint_as_float(0x7FFFFFFFu);
-        else m = fmaxf(m, fabsf(v[j]));
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-    return m;
-}
-__device__ __forceinline__ void store_any(uint8_t *row, int64_t col, int64_t ne0, const float v[4], float inv) {
-    const uint32_t lo = e4m3x2(v[0] * inv, v[1] * inv), hi = e4m3x2(v[2] * inv, v[3] * inv);
-    if (col < ne0) row[col] = (uint8_t)lo;
-    if (col + 32 < ne0) row[col + 32] = (uint8_t)(lo >> 8);
-    if (col + 64 < ne0) row[col + 64] = (uint8_t)hi;
-    if (col + 96 < ne0) row[col + 96] = (uint8_t)(hi >> 8);
-}
-
-template <int ST, typename I>
-__global__ void __launch_bounds__(256) f8_encode_rows_any_kernel(F8Codec c) {
-    constexpr int kUnits = 4;
-    const I nb = (I)((c.ne0 + kF8Block - 1) / kF8Block), total = (I)(c.n_mats * c.n_rows) * nb, rows = (I)c.n_rows;
-    const int lane = threadIdx.x & 31;
-    const I u0 = (I)blockIdx.x * (8 * kUnits) + threadIdx.x / 32;
-    float v[kUnits][4];
-    uint8_t *row[kUnits];
-    int64_t col[kUnits];
-#pragma unroll
-    for (int k = 0; k < kUnits; k++) {
-        const I u = u0 + (I)(k * 8);
-        const I g = u < total ? u / nb : 0, b = u < total ? u - g * nb : 0;
-        const I mat = c.n_mats > 1 ? g / rows : 0, r = g - mat * rows;
-        col[k] = u < total ? (int64_t)b * kF8Block + lane : c.ne0;
-        row[k] = c.codes + (int64_t)mat * c.code_mat_stride + (int64_t)r * c.code_row_stride;
-        const uint8_t *src = src_row<ST>(c, mat, r);
-#pragma unroll
-        for (int j = 0; j < 4; j++) v[k][j] = col[k] + 32 * j < c.ne0 ? load_any<ST>(src, col[k] + 32 * j) : 0.0f;
-    }
-#pragma unroll
-    for (int k = 0; k < kUnits; k++) {
-        const I u = u0 + (I)(k * 8);
-        bool inf;
-        float m = warp_top<4>(v[k], inf);
-        if (inf) m = warp_top_finite<4>(v[k]);
-        m = fmaxf(m, kF8Least);
-        store_any(row[k], col[k], c.ne0, v[k], kF8Top / m);
-        if (u < total && lane == 0) c.scales[u] = m / kF8Top;
-    }
-}
-
-// The same for a 128 x 128 tile: warp w on rows w + 8 i.
-template <int ST>
-__global__ void __launch_bounds__(256) f8_encode_tiles_any_kernel(F8Codec c) {
-    const int64_t nb = (c.ne0 + kF8Block - 1) / kF8Block, rb = (c.n_rows + kF8Block - 1) / kF8Block;
-    const int64_t tile = blockIdx.x, b = tile % nb, rest = tile / nb, mat = rest / rb;
-    const int64_t row0 = (rest - mat * rb) * kF8Block + threadIdx.x / 32;
-    const int64_t col = b * kF8Block + (threadIdx.x & 31);
-    __shared__ float s_top[2][8];
-    float v[64];
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-        const int64_t r = row0 + 8 * i;
-        const uint8_t *src = src_row<ST>(c, mat, r < c.n_rows ? r : 0);
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            v[4 * i + j] = r < c.n_rows && col + 32 * j < c.ne0 ? load_any<ST>(src, col + 32 * j) : 0.0f;
-    }
-    bool inf;
-    float m = warp_top<64>(v, inf);
-    for (int pass = 0; pass < 2; pass++) {
-        if ((threadIdx.x & 31) == 0) s_top[pass][threadIdx.x / 32] = m;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < 8; w++) m = fmaxf(m, s_top[pass][w]);
-        if (m != inf_f()) break;
-        m = warp_top_finite<64>(v);
-    }
-    m = fmaxf(m, kF8Least);
-    const float inv = kF8Top / m;
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-        const int64_t r = row0 + 8 * i;
-        if (r < c.n_rows)
-            store_any(c.codes + mat * c.code_mat_stride + r * c.code_row_stride, col, c.ne0, v + 4 * i, inv);
-    }
-    if (threadIdx.x == 0) c.scales[tile] = m / kF8Top;
-}
-
 template <typename T>
 __device__ __forceinline__ T from_f32(float v);
 template <>
@@ -347,53 +268,81 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// A warp per run of a row's columns, kEach adjacent ones a lane and step: 16
-// bytes of output where rows of the output start on 16-byte boundaries (so a
-// warp's stores are adjacent; 16 codes a lane left 64-byte strides between
-// f32 stores, 127 us for 8192 x 14336), else one.
+// A warp per run of a row's columns, 16 bytes of output a lane and step, so
+// that a warp's stores are adjacent (16 codes a lane left 64-byte strides
+// between f32 stores: 127 us for 8192 x 14336, 90 so).  Where rows of the
+// output do not all start on 16-byte boundaries (VEC false) a row's steps
+// start at its first one, their codes are shifted into place, and the few
+// elements before and after are written one by one by the run at hand.
 template <typename T, bool VEC, typename I>
 __global__ void __launch_bounds__(256) f8_decode_kernel(F8Codec c) {
-    constexpr int kEach = VEC ? 16 / (int)sizeof(T) : 1, kSteps = VEC ? 32 / kEach : 16, kRun = 32 * kEach * kSteps;
+    constexpr int kEach = 16 / (int)sizeof(T), kSteps = 32 / kEach, kRun = 32 * kEach * kSteps, kCodes = kEach / 4;
     const I runs = (I)((c.ne0 + kRun - 1) / kRun), rows = (I)c.n_rows;
     const I u = (I)blockIdx.x * 8 + threadIdx.x / 32, g = u / runs;
     if (g >= (I)(c.n_mats * c.n_rows)) return;
-    const I mat = c.n_mats > 1 ? g / rows : 0, r = g - mat * rows;
-    const int64_t col0 = (int64_t)(u - g * runs) * kRun + (threadIdx.x & 31) * kEach;
+    const I mat = c.n_mats > 1 ? g / rows : 0, r = g - mat * rows, run = u - g * runs;
+    const int lane = threadIdx.x & 31;
     const int shift = c.block_rows == 1 ? 0 : 7;
     const int64_t nb = (c.ne0 + kF8Block - 1) / kF8Block, rb = (c.n_rows + c.block_rows - 1) / c.block_rows;
     const float *scales = c.scales + ((int64_t)mat * rb + (int64_t)(r >> shift)) * nb;
     const uint8_t *codes = c.codes + (int64_t)mat * c.code_mat_stride + (int64_t)r * c.code_row_stride;
     T *out = static_cast<T *>(c.dst) + (int64_t)g * c.ne0;
-    uint32_t q[kSteps][kEach > 4 ? 2 : 1];
-    float s[kSteps];
+    // elements before the row's first 16-byte boundary
+    const int head = VEC ? 0 : (int)((16 - ((uintptr_t)out & 15) & 15) / sizeof(T));
+    const int64_t col0 = head + (int64_t)run * kRun + lane * kEach;
+    uint32_t q[kSteps][kCodes];
+    float s[kSteps][2];
 #pragma unroll
     for (int k = 0; k < kSteps; k++) {
         const int64_t col = col0 + k * 32 * kEach;
-        if (col >= c.ne0) continue;
-        s[k] = __ldg(scales + (col >> 7));
-        if (kEach == 8) {
-            const uint2 w = __ldcs(reinterpret_cast<const uint2 *>(codes + col));
-            q[k][0] = w.x;
-            q[k][kEach > 4 ? 1 : 0] = w.y;
-        } else if (kEach == 4) {
-            q[k][0] = __ldcs(reinterpret_cast<const uint32_t *>(codes + col));
+        if (col + kEach > c.ne0) continue;
+        s[k][0] = __ldg(scales + (col >> 7));
+        if (!VEC) s[k][1] = __ldg(scales + (col + kEach - 1 >> 7));
+        // whole words of codes up to the last's
+        const uint32_t *w = reinterpret_cast<const uint32_t *>(codes + (col & ~(int64_t)3));
+        if (VEC && kCodes == 2) {
+            const uint2 v = __ldcs(reinterpret_cast<const uint2 *>(w));
+            q[k][0] = v.x;
+            q[k][kCodes - 1] = v.y;
         } else {
-            q[k][0] = __ldcs(codes + col);
+            uint32_t x[kCodes + 1];
+#pragma unroll
+            for (int i = 0; i < kCodes; i++) x[i] = VEC ? __ldcs(w + i) : __ldg(w + i);
+            x[kCodes] = 0;
+            if (!VEC && (head & 3)) {
+                const int64_t at = (col & ~(int64_t)3) + 4 * kCodes;
+                if (at + 4 <= c.ne0) {
+                    x[kCodes] = __ldg(w + kCodes);
+                } else {  // nothing past the row's last code is touched
+#pragma unroll
+                    for (int i = 0; i < 3; i++)
+                        if (at + i < c.ne0) x[kCodes] |= (uint32_t)codes[at + i] << (8 * i);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kCodes; i++) q[k][i] = VEC ? x[i] : __funnelshift_r(x[i], x[i + 1], 8 * (head & 3));
         }
     }
 #pragma unroll
     for (int k = 0; k < kSteps; k++) {
         const int64_t col = col0 + k * 32 * kEach;
-        if (col >= c.ne0) continue;
-        __align__(16) T y[kEach > 1 ? kEach : 2];
+        if (col + kEach > c.ne0) continue;
+        const int in0 = VEC ? kEach : kF8Block - (int)(col & (kF8Block - 1));  // elements in the first block
+        __align__(16) T y[kEach];
 #pragma unroll
-        for (int i = 0; i < (kEach + 1) / 2; i++) {
-            const float2 f = e4m3x2_val((uint16_t)(q[k][i >> 1] >> (16 * (i & 1))));
-            y[2 * i] = from_f32<T>(f.x * s[k]);
-            y[2 * i + 1] = from_f32<T>(f.y * s[k]);
+        for (int i = 0; i < kEach; i += 2) {
+            const float2 f = e4m3x2_val((uint16_t)(q[k][i >> 2] >> (8 * (i & 2))));
+            y[i] = from_f32<T>(f.x * (VEC || i < in0 ? s[k][0] : s[k][1]));
+            y[i + 1] = from_f32<T>(f.y * (VEC || i + 1 < in0 ? s[k][0] : s[k][1]));
         }
-        if (kEach == 1) out[col] = y[0];
-        else *reinterpret_cast<uint4 *>(out + col) = *reinterpret_cast<const uint4 *>(y);
+        *reinterpret_cast<uint4 *>(out + col) = *reinterpret_cast<const uint4 *>(y);
+    }
+    if (!VEC && run == 0) {
+        const int64_t body = (c.ne0 - head) / kEach * kEach, after = c.ne0 > head ? head + body : c.ne0;
+        // lanes 0-15: the head; 16-31: what whole steps leave of the row
+        const int64_t col = lane < 16 ? lane : after + lane - 16;
+        if (lane < 16 ? lane < head && col < c.ne0 : col < c.ne0)
+            out[col] = from_f32<T>(e4m3x2_val(codes[col]).x * __ldg(scales + (col >> 7)));
     }
 }
 
@@ -403,30 +352,26 @@ unsigned grid_for(int64_t items, int64_t per_block) {
     return b > INT32_MAX ? 0 : (unsigned)b;
 }
 
-template <int ST>
-cudaError_t encode(const F8Codec &c, bool vec, cudaStream_t st) {
+template <int ST, bool VEC>
+cudaError_t encode(const F8Codec &c, cudaStream_t st) {
     const int64_t nb = (c.ne0 + kF8Block - 1) / kF8Block;
     if (c.block_rows != 1) {
         const unsigned g = grid_for(c.n_mats * ((c.n_rows + kF8Block - 1) / kF8Block) * nb, 1);
         if (!g) return cudaErrorInvalidValue;
-        if (vec) f8_encode_tiles_kernel<ST><<<g, 256, 0, st>>>(c);
-        else f8_encode_tiles_any_kernel<ST><<<g, 256, 0, st>>>(c);
+        f8_encode_tiles_kernel<ST, VEC><<<g, 256, 0, st>>>(c);
         return cudaGetLastError();
     }
     const int64_t total = c.n_mats * c.n_rows * nb;
-    const unsigned g = grid_for(total, vec ? 256 / kLanes * units<ST>() : 32);
+    const unsigned g = grid_for(total, 256 / kLanes * units<ST>());
     if (!g) return cudaErrorInvalidValue;
-    const bool wide = total >= INT32_MAX;
-    if (vec && !wide) f8_encode_rows_kernel<ST, uint32_t><<<g, 256, 0, st>>>(c);
-    else if (vec) f8_encode_rows_kernel<ST, uint64_t><<<g, 256, 0, st>>>(c);
-    else if (!wide) f8_encode_rows_any_kernel<ST, uint32_t><<<g, 256, 0, st>>>(c);
-    else f8_encode_rows_any_kernel<ST, uint64_t><<<g, 256, 0, st>>>(c);
+    if (total < INT32_MAX) f8_encode_rows_kernel<ST, VEC, uint32_t><<<g, 256, 0, st>>>(c);
+    else f8_encode_rows_kernel<ST, VEC, uint64_t><<<g, 256, 0, st>>>(c);
     return cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t decode(const F8Codec &c, bool vec, cudaStream_t st) {
-    const int64_t run = vec ? 1024 : 512, units = c.n_mats * c.n_rows * ((c.ne0 + run - 1) / run);
+    const int64_t run = 1024, units = c.n_mats * c.n_rows * ((c.ne0 + run - 1) / run);
     const unsigned g = grid_for(units, 8);
     if (!g) return cudaErrorInvalidValue;
     const bool wide = units >= INT32_MAX;
@@ -444,9 +389,9 @@ cudaError_t launch_f8_encode(const F8Codec &c, cudaStream_t st) {
     // 128-bit loads where every row starts on a 16-byte boundary
     const bool vec = ((uintptr_t)c.src & 15) == 0 && c.src_row_stride * esz % 16 == 0 &&
                      c.src_mat_stride * esz % 16 == 0;
-    if (c.type == SHC_SRC_F32) return encode<SHC_SRC_F32>(c, vec, st);
-    if (c.type == SHC_SRC_F16) return encode<SHC_SRC_F16>(c, vec, st);
-    return encode<SHC_SRC_BF16>(c, vec, st);
+    if (c.type == SHC_SRC_F32) return vec ? encode<SHC_SRC_F32, true>(c, st) : encode<SHC_SRC_F32, false>(c, st);
+    if (c.type == SHC_SRC_F16) return vec ? encode<SHC_SRC_F16, true>(c, st) : encode<SHC_SRC_F16, false>(c, st);
+    return vec ? encode<SHC_SRC_BF16, true>(c, st) : encode<SHC_SRC_BF16, false>(c, st);
 }
 
 cudaError_t launch_f8_decode(const F8Codec &c, cudaStream_t st) {

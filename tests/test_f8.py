@@ -160,6 +160,28 @@ def test_decode_is_code_times_scale(ctx, shape, dtype, block_rows):
     assert got.is_contiguous() and torch.equal(got, (codes.float() * s).to(dtype))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=str)
+@pytest.mark.parametrize("cols", [1, 3, 9, 127, 129, 1023, 1030, 2051])
+def test_decode_and_encode_at_every_alignment(ctx, dtype, cols):
+    """Outputs and sources that start at any element: no row on a 16-byte boundary but by chance."""
+    g = gen(cols)
+    codes, scales = ctx.encode_f8(rand(g, 5, cols))
+    s = scales.repeat_interleave(128, -1)[:, :cols]
+    for left in range(9):
+        buf = torch.full((5 * cols + 32,), 3.0, dtype=dtype, device="cuda")
+        out = buf[left:left + 5 * cols].view(5, cols)
+        ctx.decode_f8(codes, scales, dtype=dtype, out=out, sync=True)
+        assert torch.equal(out, (codes.float() * s).to(dtype))
+        x = out.clone()
+        out.copy_(rand(g, 5, cols))
+        for block_rows in (1, 128):
+            want, ws = plain_encode(out, block_rows)
+            got, gs = ctx.encode_f8(out, block_rows, sync=True)
+            assert torch.equal(got.view(torch.uint8), want) and torch.equal(gs, ws)
+        out.fill_(3.0)
+        assert (buf == 3.0).all() and x.shape == out.shape
+
+
 def test_decode_every_code(ctx):
     codes = torch.arange(256, dtype=torch.uint8, device="cuda").view(2, 128)
     got = ctx.decode_f8(codes, torch.ones(2, 1, device="cuda"), sync=True)
