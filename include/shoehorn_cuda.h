@@ -197,7 +197,7 @@ int shc_encode_rows_noalloc(uint32_t ggml_type, uint32_t src_type, const void *s
  * strides are multiples of 16 bytes; bytes between the rows' ends and the
  * next rows are neither read as values nor written.  Scales are dense:
  * [n_mats, ceil(n_rows / block_rows), ceil(ne0 / 128)].  Rows, columns and
- * matrices are below 2^31 each.  Strides count elements (bytes for codes).
+ * matrices are at most 2^31 - 1024 each.  Strides count elements (bytes for codes).
  * Outputs may not overlap inputs. */
 
 /* Encode n_mats matrices of n_rows rows (device pointers); source rows may
@@ -218,8 +218,8 @@ int shc_decode_f8(shc_ctx *ctx, uint32_t dst_type, const uint8_t *codes, int64_t
  *                 A W^T's result as A, the gradient of its rows
  * A is encoded with block_rows 1; its scales are a_scale_stride apart from
  * row to row.  Each block's 128 products are summed in f32 and scaled by the
- * f32 product of the two scales; blocks are summed in order in f32, and the
- * sum is rounded once to dst_type (SHC_SRC_*). */
+ * f32 product of the two scales; blocks are summed in f32, in an order that
+ * the sizes alone decide, and the sum is rounded once to dst_type (SHC_SRC_*). */
 int shc_matmul_f8(shc_ctx *ctx, const uint8_t *a, int64_t a_row_stride, const float *a_scales, int64_t a_scale_stride,
                   int64_t n_rows, const uint8_t *w, int64_t w_row_stride, const float *w_scales, int64_t n, int64_t k,
                   int transposed, uint32_t dst_type, void *dst, int64_t dst_row_stride, void *stream);

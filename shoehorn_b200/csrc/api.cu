@@ -272,7 +272,7 @@ bool is_pinned(const void *p) {
 // A matrix (or n_mats of them) of 8-bit codes: rows on 16-byte boundaries,
 // and sizes that TMA coordinates and strides can hold.
 bool f8_codes_ok(const void *p, int64_t n_mats, int64_t n_rows, int64_t cols, int64_t row_stride, int64_t mat_stride) {
-    constexpr int64_t kMaxDim = INT32_MAX, kMaxStride = (int64_t)1 << 40;
+    constexpr int64_t kMaxDim = INT32_MAX - 1023, kMaxStride = (int64_t)1 << 40;  // a tile may end past the last row
     if (n_mats > kMaxDim || n_rows > kMaxDim || cols < 1 || cols > kMaxDim) return false;
     if (((uintptr_t)p & 15) != 0 || row_stride % 16 != 0 || row_stride < cols || row_stride >= kMaxStride) return false;
     if (n_mats > 1 && (mat_stride % 16 != 0 || mat_stride >= kMaxStride || mat_stride / row_stride < n_rows - 1 ||

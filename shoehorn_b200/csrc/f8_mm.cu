@@ -884,19 +884,47 @@ int64_t most_tiles(const MmArgs &a, int tm, int bn) {
     return (((int64_t)a.n_rows + tm - 1) / tm + (a.offsets ? some : 0)) * ((a.out + bn - 1) / bn);
 }
 
-// CTAs to share a tile's contraction where the tiles alone leave most SMs
-// idle.  Measured (1 to 256 rows, 1024 to 4096 columns, 8 to 112 blocks): a
-// block takes 0.28 us, joining two parts 1.7 us + 3.5 us x rows / 128 and
-// four or eight 1.3 + 2.8 x rows / 128, whatever the number of blocks.  So one
-// row through 4096 x 4096 takes 8.7 us in four parts (13.4 in one), 128 rows
-// through 2048 x 1024 8.1 (6.1 in one: not split).  Clusters of eight do not
-// all run at once beyond 64 CTAs (16 of them take twice as long as 8).
-int split_for(int64_t tiles, int blocks, int rows, int num_sms) {
-    int best = 1, least = 28 * blocks;
+// Which tiles to use: the least of the times below, in units of 10 ns, fitted
+// to 60 products of 1 to 8192 rows, 1024 to 14336 columns and 8 to 112 blocks
+// (within 15 % of all but those that HBM bounds, where the shapes tie).
+//
+//   tile                    start   each wave of tiles        4096 cubed, measured
+//   128 x 128               3.9 us  1.0 us + 0.29 x blocks    79 us
+//   128 x 256               3.5     2.0    + 0.47             71
+//   256 x 256, CTA pair     3.0     3.4    + 0.41             68
+//
+// A grouped product has row tiles for whole tiles' rows and half a tile more
+// for each expert, or one for each expert with rows.  Where 128 x 128 tiles
+// leave most SMs idle, a cluster of CTAs shares a tile's contraction: joining
+// two parts takes 1.7 us + 3.5 x rows / 128 and four or eight 1.3 + 2.8 x rows
+// / 128, whatever the number of blocks, so that one row through 4096 x 4096
+// takes 8.7 us in four parts (13.4 in one) and 128 rows through 2048 x 1024 6.1
+// in one (8.1 in four).  Clusters of eight do not all run at once beyond 64
+// CTAs (16 of them take twice as long as 8).
+struct Plan {
+    int bn, pair, split;
+};
+Plan plan_for(const MmArgs &a, int num_sms) {
+    const auto waves = [&](int tm, int bn, int at_once) {
+        int64_t down = ((int64_t)a.n_rows + tm - 1) / tm;
+        if (a.offsets) {
+            const int64_t some = a.n_experts < a.n_rows ? a.n_experts : a.n_rows;
+            down = down + some / 2 > some ? down + some / 2 : some;
+        }
+        return (down * ((a.out + bn - 1) / bn) + at_once - 1) / at_once;
+    };
+    const int64_t c = a.blocks_c;
+    Plan best{128, 1, 1};
+    int64_t least = 390 + waves(128, 128, num_sms) * (100 + 29 * c);
+    const auto offer = [&](int64_t time, Plan plan) {
+        if (time < least) least = time, best = plan;
+    };
+    offer(350 + waves(128, 256, num_sms) * (200 + 47 * c), Plan{256, 1, 1});
+    offer(300 + waves(256, 256, num_sms / 2) * (340 + 41 * c), Plan{256, 2, 1});
+    const int64_t tiles = most_tiles(a, kTileM, 128), each = a.n_rows / a.n_experts, rows = each < kTileM ? each : kTileM;
     for (int z = 2; z <= 8; z *= 2) {
-        if (tiles * z > (z == 8 ? 64 : num_sms) || blocks < 2 * z) break;
-        const int time = 28 * blocks / z + (z == 2 ? 170 + 350 * rows / 128 : 130 + 280 * rows / 128);
-        if (time < least) least = time, best = z;
+        if (tiles * z > (z == 8 ? 64 : num_sms) || c < 2 * z) break;
+        offer(490 + 29 * c / z + (z == 2 ? 170 + 350 * rows / 128 : 130 + 280 * rows / 128), Plan{128, 1, z});
     }
     return best;
 }
@@ -933,8 +961,7 @@ int launch_f8_product(const F8Product &p, int num_sms, cudaStream_t st) {
     const uint64_t starts = (uintptr_t)p.dst | (uint64_t)(p.dst_row_stride * esz);
     a.align = starts % 16 == 0 ? 16 : starts % 8 == 0 ? 8 : 1;
     a.status = p.status;
-    const int64_t rows_each = p.n_rows / p.n_experts;
-    a.a_box = rows_each >= kTileM ? kTileM : 32;
+    a.a_box = p.n_rows / p.n_experts >= kTileM ? kTileM : 32;  // short experts: no more rows than there are, nearly
 
     CUtensorMap maps[3];
     if (!code_map(&maps[0], p.a, inner, p.n_rows, 1, p.a_row_stride, 0, a.a_box, 2) ||
@@ -943,15 +970,15 @@ int launch_f8_product(const F8Product &p, int num_sms, cudaStream_t st) {
     a.tma_store = a.align == 16 && p.dst_row_stride * esz < ((int64_t)1 << 40) &&
                   out_map(&maps[2], p.dst, out, p.n_rows, p.dst_row_stride, p.dst_type);
     if (!a.tma_store) maps[2] = maps[0];
-    // Wide tiles where they fill the machine, in pairs where an expert has rows for several.
-    const int64_t each = (rows_each + kTileM - 1) / kTileM * p.n_experts, wide = each * ((out + 255) / 256);
+    const Plan plan = plan_for(a, num_sms);
+    a.split = plan.split;
     cudaError_t e;
-    a.split = split_for(most_tiles(a, kTileM, 128), a.blocks_c, (int)(rows_each < kTileM ? rows_each : kTileM), num_sms);
-    if (a.split > 1) e = launch_shape<128, 1, true>(maps, a, p.transposed, num_sms, st);
-    else if (wide >= num_sms && rows_each >= 1024) e = launch_shape<256, 2>(maps, a, p.transposed, num_sms, st);
-    else if (wide >= num_sms && rows_each >= kTileM) e = launch_shape<256, 1>(maps, a, p.transposed, num_sms, st);
+    if (plan.pair == 2) e = launch_shape<256, 2>(maps, a, p.transposed, num_sms, st);
+    else if (plan.bn == 256) e = launch_shape<256, 1>(maps, a, p.transposed, num_sms, st);
+    else if (plan.split > 1) e = launch_shape<128, 1, true>(maps, a, p.transposed, num_sms, st);
     else e = launch_shape<128, 1>(maps, a, p.transposed, num_sms, st);
     if (e == cudaSuccess) return SHC_OK;
+    cudaGetLastError();  // reported here; the next call's launch check starts clean
     return e == cudaErrorMemoryAllocation ? SHC_ENOMEM : SHC_ECUDA;
 }
 
