@@ -9,14 +9,17 @@ tensor core's, so each of at most 128 additions is allowed one f32 step,
 once to the output type (eps / 2): |D - exact| <= (128 * 2^-23 + (blocks + 2)
 * 2^-24) * S + eps / 2 * |exact| (+ half a subnormal step of f16)."""
 import math
+import os
+import subprocess
+import sys
 
-import numpy as np
 import pytest
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 import shoehorn_b200 as sh  # noqa: E402
 
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 TOP, LEAST = 448.0, 448.0 * 2.0**-126
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 
@@ -212,6 +215,36 @@ def test_product(ctx, m, n, k, transposed):
         got = ctx.matmul_f8(a, sa, w, sw, transposed=transposed, dtype=dtype, sync=True)
         assert got.dtype == dtype and got.shape == (m, k if transposed else n)
         check_product(got, a, sa, w, sw, transposed)
+
+
+SHAPES_OF_TILES = [  # rows, outputs, contraction, experts: sizes that the kernel's tile shapes are chosen for
+    (1, 1030, 1100, 0), (3, 700, 2100, 0), (130, 1000, 4200, 0),  # contraction shared by four and eight CTAs
+    (40, 5000, 2500, 0), (1, 9000, 5100, 0),  # by two
+    (300, 2500, 3800, 0), (2000, 2049, 600, 0), (2047, 4100, 4090, 0),  # 128 x 128, 128 x 256, pairs
+    (300, 200, 2500, 3), (20, 300, 4200, 2), (5000, 1000, 1100, 8), (2000, 1000, 1100, 8), (9000, 4100, 4090, 4),
+]
+
+
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("rows,out,inner,experts", SHAPES_OF_TILES)
+def test_every_tile_shape(ctx, rows, out, inner, experts, transposed):
+    g = gen(rows + out)
+    n, k = (inner, out) if transposed else (out, inner)
+    a, sa = encoded(ctx, g, rows, inner, 1)
+    for dtype, pad in ((F32, 0), (BF16, 3), (F16, 16)):
+        buf = torch.full((rows, out + pad), 3.0, dtype=dtype, device="cuda")
+        got = buf[:, :out]
+        if experts:
+            w, sw = ctx.encode_f8(rand(g, experts, n, k) * 0.05, 128)
+            at = torch.sort(torch.randint(rows + 1, (experts + 1,), generator=g, device="cuda"))[0]
+            before = got.clone()
+            ctx.matmul_f8_grouped(a, sa, w, sw, at, transposed=transposed, out=got, sync=True)
+            check_grouped(got, before, a, sa, w, sw, at, transposed)
+        else:
+            w, sw = encoded(ctx, g, n, k, 128, 0.05)
+            ctx.matmul_f8(a, sa, w, sw, transposed=transposed, out=got, sync=True)
+            check_product(got, a, sa, w, sw, transposed)
+        assert (buf[:, out:] == 3.0).all()
 
 
 def test_no_rows(ctx):
@@ -462,6 +495,31 @@ def test_captured_and_replayed(ctx):
             assert torch.equal(a.view(torch.uint8), want) and torch.equal(sa, ws)
             check_grouped(d, d, a, sa, w, sw, offsets, False)
             check_product(one, a[:1], sa[:1], w[0], sw[0], False)
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    """Nothing that a first call sets up keeps it out of a graph."""
+    code = """
+import torch, shoehorn_b200 as sh
+ctx = sh.Context(0)
+x = torch.randn(200, 384, device="cuda")
+w = torch.randn(256, 384, device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    a, sa = ctx.encode_f8(x)
+    b, sb = ctx.encode_f8(w, 128)
+    d = ctx.matmul_f8(a, sa, b, sb, dtype=torch.float32)
+    e = ctx.matmul_f8(a[:1], sa[:1], b, sb, dtype=torch.float32)
+graph.replay()
+torch.cuda.synchronize()
+ctx.sync()
+want = ctx.decode_f8(a, sa).double() @ ctx.decode_f8(b, sb, 128).double().t()
+assert (d - want).abs().max() < 1e-4 * want.abs().max(), (d - want).abs().max()
+assert torch.equal(d[:1], e) or (d[:1] - e).abs().max() < 1e-4 * want.abs().max()
+print("captured")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=ROOT)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stdout + r.stderr
 
 
 def test_experts_from_quantised_tensors(ctx):
