@@ -159,6 +159,7 @@ class Context:
     def __init__(self, device=0):
         import torch  # device memory and streams are torch's
         self.torch = torch
+        self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         self.device = int(device)
         h = ctypes.c_void_p()
         _check(lib().shc_init(self.device, ctypes.byref(h)), "shc_init")
@@ -294,7 +295,7 @@ class Context:
         return stream.cuda_stream, torch.cuda.stream(stream)
 
     def _f8_stream(self):
-        raw = getattr(self.torch._C, "_cuda_getCurrentRawStream", None)
+        raw = self._raw_stream  # torch's own accessor of the handle, ten times faster than a Stream object
         return raw(self.device) if raw else self.torch.cuda.current_stream(self.device).cuda_stream
 
     def _f8_here(self, t, what):
@@ -426,9 +427,14 @@ class Context:
             if out.dtype is not dtype or out.shape != shape or not out.is_contiguous():
                 raise ValueError("out must be contiguous, of codes' shape and of dtype")
 
-        stp, on = self._f8_on(stream, codes, scales, out)
-        with on:
-            res = codes.new_empty(shape, dtype=dtype) if out is None else out
+        if stream is None:
+            stp, res = self._f8_stream(), out
+            if out is None:
+                res = codes.new_empty(shape, dtype=dtype)
+        else:
+            stp, on = self._f8_on(stream, codes, scales, out)
+            with on:
+                res = codes.new_empty(shape, dtype=dtype) if out is None else out
         rc = lib().shc_decode_f8(self.handle, dt, codes.data_ptr(), mats, rows, cols, pitch, step, block_rows,
                                  scales.data_ptr(), res.data_ptr(), stp)
         if rc:
@@ -460,9 +466,14 @@ class Context:
             if (cols > 1 and out.stride(1) != 1) or pitch_o < cols:
                 raise ValueError("out's columns must be adjacent and its rows apart")
 
-        stp, on = self._f8_on(stream, a, a_scales, w, w_scales, offsets, out)
-        with on:
-            res = a.new_empty((rows, cols), dtype=dtype) if out is None else out
+        if stream is None:
+            stp, res = self._f8_stream(), out
+            if out is None:
+                res = a.new_empty((rows, cols), dtype=dtype)
+        else:
+            stp, on = self._f8_on(stream, a, a_scales, w, w_scales, offsets, out)
+            with on:
+                res = a.new_empty((rows, cols), dtype=dtype) if out is None else out
         if offsets is None:
             rc = lib().shc_matmul_f8(self.handle, a.data_ptr(), pitch_a, a_scales.data_ptr(), pitch_s, rows, w.data_ptr(),
                                      pitch_w, w_scales.data_ptr(), n, k, transposed, dt, res.data_ptr(), pitch_o, stp)
@@ -562,11 +573,15 @@ def default_context(device=None):
     """Process-wide context on the current CUDA device (like the reference's
     process-wide OnceLock grids)."""
     global _default_ctx
-    import torch
+    ctx = _default_ctx
+    if ctx is None:
+        import torch
+    else:
+        torch = ctx.torch
     dev = torch.cuda.current_device() if device is None else device
-    if _default_ctx is None or _default_ctx.device != dev:
-        _default_ctx = Context(dev)
-    return _default_ctx
+    if ctx is None or ctx.device != dev:
+        ctx = _default_ctx = Context(dev)
+    return ctx
 
 
 # ---------------- reference row API (quant.rs:543-630) ----------------
