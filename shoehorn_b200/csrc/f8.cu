@@ -9,6 +9,12 @@
 // element, so a code's value before its rounding to E4M3 is within 2^-23 of
 // x / scale.  NaN and infinite elements become the NaN code and leave the
 // block's scale to the finite ones.
+//
+// All three kernels are bound by HBM: an element is read once and its code
+// written once (the tile kernel holds its tile in registers between the
+// maximum and the codes).  8192 x 14336 bf16 to 1 x 128 blocks 62.5 us (5.69
+// TB/s, 0.87 of the measured copy), to tiles 60.5, f32 87-91 us (6.5-6.8
+// TB/s); 14336 x 4096 tiles decoded to bf16 28.7 us (6.15 TB/s, 0.94).
 #include "f8.cuh"
 
 namespace shc {

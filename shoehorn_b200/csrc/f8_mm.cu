@@ -11,12 +11,34 @@
 // it, scaled, into f32 registers.  Nothing is rounded below f32 before the
 // final conversion to the output type.
 //
-// A CTA computes 128 rows x BN columns at a time.  One warp keeps a ring of
-// shared-memory stages filled by TMA (128 contraction bytes per row, 128-byte
-// swizzle), one thread issues the tcgen05 products of a stage into one of two
-// TMEM accumulators, and BN / 32 epilogue warps drain the other.  W is read
-// in the same boxes for both products; only its descriptor differs (K-major
-// for W^T, MN-major for W).
+// Twelve warps, each with one job:
+//   loads     TMA into a ring of stages: 128 contraction bytes of A's and B's
+//             rows, 128-byte swizzle.  W is read in the same boxes for both
+//             products; only its descriptor differs (K-major for W^T, MN-major
+//             for W).
+//   products  two warps issue the even and the odd blocks (tcgen05.mma,
+//             kind::f8f6f4), every block into an accumulator of its own.
+//   scales    one warp multiplies sa by sb for four blocks at a time and hands
+//             them to the epilogue through shared memory, with the tile's
+//             place (scales loaded by the epilogue itself stalled it: 401
+//             against 309 us for 4096 x 14336 x 4096).
+//   epilogue  eight warps drain the accumulators (two per 128 columns, so one
+//             fills while the other is read) and store the tile through TMA.
+// Tiles are 128 x 128, 128 x 256, or 256 x 256 by a pair of CTAs (each holds
+// its own 128 rows of A and half of B, so a block takes 32 KB from L2 per CTA
+// where a single one takes 48); plan_for says when.  Where few tiles leave
+// SMs idle, a cluster shares a tile's contraction and joins its sums through
+// distributed shared memory, in rank order: no atomics, no workspace.
+//
+// What bounds it (4096 x 14336 x 4096, a pair's 256 x 256 tiles, 217-245 us by
+// box, 1.96-2.2 PFLOP/s, clocks at 1.57 GHz under the power limit): the
+// products alone take 138 us (514 cycles a block, their rate), the loads
+// alone 113 us (17 TB/s from L2), but a block passes in 865 cycles, because
+// an epilogue warp needs that long to wait for, read and scale its 128
+// columns; without the scaling it is 620, without the stores 785.  Sixteen
+// narrower epilogue warps took 247 us (more instructions), 32-column TMEM
+// loads 290 (spilled), a single warp issuing products and acknowledging on
+// two barriers a block 301.
 //
 // Rows of an expert (or of the whole matrix) that lie past its end are loaded
 // as zeros or as the next expert's rows, and not stored: rows of D depend on

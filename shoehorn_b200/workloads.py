@@ -54,18 +54,26 @@ def main(argv=None):
       python -m shoehorn_b200.workloads --type 14 --rows 512 [--dist iq] [--repeat 2]
 
     --table STEP computes the fused error table (row_errors) of every STEP-th
-    row instead of encoding.
+    row instead of encoding.  --product M encodes the tensor to 8-bit blocks
+    and multiplies M rows of activations by it instead (--transposed: M rows
+    of gradients, back through it):
+
+      python -m shoehorn_b200.workloads --product 4096 --rows 4096 --dist iq
     """
     import argparse
     ap = argparse.ArgumentParser(prog="python -m shoehorn_b200.workloads")
-    ap.add_argument("--type", type=int, required=True, help="ggml type id")
+    ap.add_argument("--type", type=int, help="ggml type id (needed without --product)")
     ap.add_argument("--rows", type=int, default=512)
     ap.add_argument("--dist", choices=["sweep", "iq"], default="sweep",
                     help="sweep: N(0, 0.02) + outliers, 14336 wide; iq: Student-t, 4096 wide")
     ap.add_argument("--repeat", type=int, default=2)
     ap.add_argument("--table", type=int, default=0, metavar="STEP",
                     help="fused error table of every STEP-th row instead of the encode")
+    ap.add_argument("--product", type=int, default=0, metavar="M", help="8-bit product of M rows instead of the encode")
+    ap.add_argument("--transposed", action="store_true", help="with --product: the gradient's direction")
     args = ap.parse_args(argv)
+    if args.type is None and not args.product:
+        ap.error("--type or --product is needed")
     import torch
     import shoehorn_b200 as sh
     if args.dist == "sweep":
@@ -77,6 +85,15 @@ def main(argv=None):
     with sh.Context(0) as ctx:
         src = torch.from_numpy(bits.view(np.int16)).cuda()
         imt = torch.from_numpy(im).cuda()
+        if args.product:
+            w, ws = ctx.encode_f8(src.view(torch.bfloat16), block_rows=128)
+            g = torch.Generator(device="cuda").manual_seed(SEED)
+            x = torch.randn(args.product, w.shape[0 if args.transposed else 1], generator=g, device="cuda")
+            for _ in range(args.repeat):
+                a, s = ctx.encode_f8(x)
+                ctx.matmul_f8(a, s, w, ws, transposed=args.transposed, sync=True)
+            print(f"multiplied {args.product} rows by {args.rows} x {bits.shape[1]} in 8-bit blocks x{args.repeat}")
+            return
         for _ in range(args.repeat):
             if args.table:
                 ctx.row_errors([args.type], src, imt, row_step=args.table, sync=True)
