@@ -389,6 +389,10 @@ class Context:
         pitch = (cols + 15) // 16 * 16
         step = rows * pitch
 
+        if out is not None:
+            pitch, step = self._f8_codes(out, "out", (2, 3))[3:]
+        if scales is not None:
+            self._f8_scales(scales, "scales", blocks)
         stp, on = self._f8_on(stream, src, out, scales)
         with on:
             codes, made = out, scales
@@ -398,10 +402,6 @@ class Context:
                     codes = codes[..., :cols]
             if made is None:
                 made = src.new_empty(blocks, dtype=torch.float32)
-        if out is not None:
-            pitch, step = self._f8_codes(out, "out", (2, 3))[3:]
-        if scales is not None:
-            self._f8_scales(scales, "scales", blocks)
         rc = lib().shc_encode_f8(self.handle, st, src.data_ptr(), mats, rows, cols, stride[-2] if rows > 1 else cols,
                                  stride[0] if mats > 1 else 0, block_rows, codes.data_ptr(), pitch, step,
                                  made.data_ptr(), stp)

@@ -118,3 +118,13 @@ def test_shapes_and_layouts_that_are_refused(rec):
         with pytest.raises(kind):
             call()
     assert not rec.calls
+
+
+def test_given_outputs_are_checked_before_a_stream_is_asked_to_keep_them(rec, monkeypatch):
+    ctx = CpuContext()
+    asked = []
+    monkeypatch.setattr(ctx, "_f8_on", lambda *a: asked.append(a), raising=False)
+    for kw in ({"out": torch.zeros(4, 8, dtype=torch.uint8)}, {"scales": torch.zeros(4, 2)}):
+        with pytest.raises(ValueError):
+            ctx.encode_f8(torch.zeros(4, 8), **kw)
+    assert not asked and not rec.calls
