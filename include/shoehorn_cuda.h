@@ -229,8 +229,9 @@ int shc_matmul_f8(shc_ctx *ctx, const uint8_t *a, int64_t a_row_stride, const fl
  * of n_experts + 1 non-decreasing int32 (or, with offsets_64, int64) values,
  * read when the work runs; an expert may have no rows.  Rows before
  * offsets[0] and from offsets[n_experts] on are left as they are in dst.
- * Offsets outside [0, n_rows] are read as the nearest of the two, and an
- * expert whose offsets decrease has no rows. */
+ * Offsets outside [0, n_rows] are read as the nearest of the two, and one
+ * below an earlier offset as the largest before it, so that a row has one
+ * expert at most. */
 int shc_matmul_f8_grouped(shc_ctx *ctx, const uint8_t *a, int64_t a_row_stride, const float *a_scales,
                           int64_t a_scale_stride, int64_t n_rows, const uint8_t *w, int64_t w_row_stride,
                           int64_t w_mat_stride, const float *w_scales, int64_t n_experts, int64_t n, int64_t k,

@@ -35,7 +35,8 @@
 // products alone take 138 us (514 cycles a block, their rate), the loads
 // alone 113 us (17 TB/s from L2), but a block passes in 865 cycles, because
 // an epilogue warp needs that long to wait for, read and scale its 128
-// columns; without the scaling it is 620, without the stores 785.  Sixteen
+// columns.  With one multiply-add in eight it took 202 us, without the stores
+// 217, without either 164 (where the whole took 227).  Sixteen
 // narrower epilogue warps took 247 us (more instructions), 32-column TMEM
 // loads 290 (spilled), a single warp issuing products and acknowledging on
 // two barriers a block 301.
@@ -335,15 +336,17 @@ struct Tile {
 // Hands out tiles of TM x BN to the grid's CTAs (or pairs) in turn: expert by expert, within an
 // expert a column of row tiles before the next column (so CTAs running
 // together share W's tiles in L2).  Called by whole warps; experts are looked
-// up 32 at a time.  Offsets are clamped to the rows there are, so no tile
-// reaches outside A and D whatever they hold.
+// up 32 at a time.  Offsets are clamped to the rows there are and to the
+// largest one before them, so that whatever they hold no tile reaches outside
+// A and D, no row is in two tiles, and there are most_tiles at most (a cluster
+// that shares a contraction takes one tile only: its sums lie in the ring).
 template <int BN, int PAIR>
 struct Tiles {
     static constexpr int TM = kTileM * PAIR;
     int64_t t, base;  // base: tiles before expert e0
-    int e0;
+    int e0, least;   // least: the largest offset before e0's
     const MmArgs &p;
-    __device__ __forceinline__ Tiles(const MmArgs &args) : t(blockIdx.x / (PAIR * args.split)), base(0), e0(0), p(args) {}
+    __device__ __forceinline__ Tiles(const MmArgs &args) : t(blockIdx.x / (PAIR * args.split)), base(0), e0(0), least(0), p(args) {}
     __device__ __forceinline__ int offset(int e) const {
         const int64_t v = p.offsets_64 ? static_cast<const int64_t *>(p.offsets)[e]
                                        : (int64_t) static_cast<const int32_t *>(p.offsets)[e];
@@ -359,8 +362,15 @@ struct Tiles {
                 const int e = e0 + lane;
                 lo = e < p.n_experts ? offset(e) : 0;
                 hi = e < p.n_experts ? offset(e + 1) : 0;
+                if (__any_sync(~0u, e < p.n_experts && (lo < least || hi < lo))) {  // offsets that decrease
+                    lo = lo < least ? least : lo;
+                    for (int d = 1; d < 32; d <<= 1) {
+                        const int v = __shfl_up_sync(~0u, lo, d);
+                        if (lane >= d && v > lo) lo = v;
+                    }
+                    if (hi < lo) hi = lo;
+                }
             }
-            if (hi < lo) hi = lo;
             const int64_t mine = (int64_t)(((uint32_t)(hi - lo) + TM - 1) / TM) * n_out;
             int64_t sum = mine;  // inclusive prefix sum over the lanes
             for (int d = 1; d < 32; d <<= 1) {
@@ -382,6 +392,7 @@ struct Tiles {
                 return true;
             }
             base += __shfl_sync(~0u, sum, 31);
+            least = __shfl_sync(~0u, hi, 31);  // of 32 experts; with fewer this was the last look
             e0 += 32;
         }
     }

@@ -395,6 +395,44 @@ def test_grouped_many_experts(ctx, experts, rows, n, k, transposed):
     check_grouped(got, got, a, sa, w, sw, offsets, transposed)
 
 
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("rows,n,k,experts,at", [
+    (100, 1000, 2500, 8, [0, 60, 10, 70, 10, 80, 10, 90, 10]),  # contraction shared by a cluster,
+    (100, 2500, 1000, 8, [0, 60, 10, 70, 10, 80, 10, 90, 10]),  # transposed too
+    (300, 256, 200, 5, [0, 200, 50, 250, 0, 300]),
+    (500, 130, 257, 70, None),  # more experts than are looked up at once
+    (3000, 1024, 1100, 6, [0, 2000, 100, 2500, 100, 2700, 3000]),
+])
+def test_grouped_offsets_that_fall_and_rise(ctx, rows, n, k, experts, at, transposed):
+    """An offset below an earlier one is read as the largest before it: no row has two experts."""
+    g = gen(rows + experts)
+    a, sa = encoded(ctx, g, rows, n if transposed else k, 1)
+    w, sw = ctx.encode_f8(rand(g, experts, n, k) * 0.05, 128)
+    if at is None:
+        offsets = torch.randint(rows + 1, (experts + 1,), generator=g, device="cuda") * torch.arange(experts + 1, device="cuda") // experts
+    else:
+        offsets = torch.tensor(at, dtype=torch.int32, device="cuda")
+    before = torch.full((rows, k if transposed else n), 3.0, device="cuda")
+    out = before.clone()
+    ctx.matmul_f8_grouped(a, sa, w, sw, offsets, transposed=transposed, out=out, sync=True)
+    check_grouped(out, before, a, sa, w, sw, torch.cummax(offsets, 0)[0], transposed)
+
+
+@pytest.mark.parametrize("transposed", [False, True])
+def test_grouped_weights_a_part_row_apart(ctx, transposed):
+    """Matrices whose distance is neither a multiple of the row pitch nor whole rows."""
+    g = gen(9)
+    experts, n, k, rows, pitch = 3, 30, 100, 90, 256
+    step = (n - 1) * pitch + 112
+    a, sa = encoded(ctx, g, rows, n if transposed else k, 1)
+    w, sw = ctx.encode_f8(rand(g, experts, n, k) * 0.05, 128)
+    apart = torch.zeros(experts * step + pitch, dtype=torch.uint8, device="cuda").as_strided((experts, n, k), (step, pitch, 1))
+    apart.copy_(w.view(torch.uint8))
+    offsets = torch.tensor([0, 20, 60, 90], device="cuda")
+    got = ctx.matmul_f8_grouped(a, sa, apart, sw, offsets, transposed=transposed, dtype=F32, sync=True)
+    check_grouped(got, got, a, sa, w, sw, offsets, transposed)
+
+
 def test_grouped_weights_apart(ctx):
     """Experts' weights some distance from one another, and only some of them."""
     g = gen(9)
