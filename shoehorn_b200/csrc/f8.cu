@@ -12,9 +12,10 @@
 //
 // All three kernels are bound by HBM: an element is read once and its code
 // written once (the tile kernel holds its tile in registers between the
-// maximum and the codes).  8192 x 14336 bf16 to 1 x 128 blocks 62.5 us (5.69
-// TB/s, 0.87 of the measured copy), to tiles 60.5, f32 87-91 us (6.5-6.8
-// TB/s); 14336 x 4096 tiles decoded to bf16 28.7 us (6.15 TB/s, 0.94).
+// maximum and the codes).  8192 x 14336 bf16 to 1 x 128 blocks 63.2 us (5.63
+// TB/s, 0.86 of the measured copy), to tiles 60.8, f32 87-91 us (6.5-6.8
+// TB/s); 14336 x 4096 tiles decoded to bf16 28.6 us (6.16 TB/s, 0.94).  Rows
+// that start off 16-byte boundaries: 8192 x 14330 bf16 97 us, f32 101.
 #include "f8.cuh"
 
 namespace shc {

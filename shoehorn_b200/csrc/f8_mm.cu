@@ -30,8 +30,8 @@
 // SMs idle, a cluster shares a tile's contraction and joins its sums through
 // distributed shared memory, in rank order: no atomics, no workspace.
 //
-// What bounds it (4096 x 14336 x 4096, a pair's 256 x 256 tiles, 217-245 us by
-// box, 1.96-2.2 PFLOP/s, clocks at 1.57 GHz under the power limit): the
+// What bounds it (4096 x 14336 x 4096, a pair's 256 x 256 tiles, 221-250 us,
+// 1.93-2.18 PFLOP/s, with the clock that the power limit leaves): the
 // products alone take 138 us (514 cycles a block, their rate), the loads
 // alone 113 us (17 TB/s from L2), but a block passes in 865 cycles, because
 // an epilogue warp needs that long to wait for, read and scale its 128
@@ -931,7 +931,7 @@ int64_t most_tiles(const MmArgs &a, int tm, int bn) {
 // leave most SMs idle, a cluster of CTAs shares a tile's contraction: joining
 // two parts takes 1.7 us + 3.5 x rows / 128 and four or eight 1.3 + 2.8 x rows
 // / 128, whatever the number of blocks, so that one row through 4096 x 4096
-// takes 8.7 us in four parts (13.4 in one) and 128 rows through 2048 x 1024 6.1
+// takes 8.7 us in four parts (13.2 in one) and 128 rows through 2048 x 1024 6.1
 // in one (8.1 in four).  Clusters of eight do not all run at once beyond 64
 // CTAs (16 of them take twice as long as 8).
 struct Plan {
