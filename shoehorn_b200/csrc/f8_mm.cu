@@ -163,12 +163,16 @@ __device__ __forceinline__ bool elect_one() {
     return one != 0;
 }
 // For a whole warp: one try by all lanes, then one lane waits for all (32
-// pollers a barrier slow the others down).
+// pollers a barrier slow the others down).  The lanes that did not see the
+// phase complete themselves are ordered behind the one that did by
+// __syncwarp; the shuffle alone orders no memory.
 __device__ __forceinline__ bool warp_wait(unsigned long long *b, uint32_t parity, volatile int *abort, int *status) {
     if (__all_sync(~0u, bar_test(b, parity))) return true;
     int ok = 1;
     if ((threadIdx.x & 31) == 0) ok = bar_wait(b, parity, abort, status);
-    return __shfl_sync(~0u, ok, 0);
+    ok = __shfl_sync(~0u, ok, 0);
+    __syncwarp();
+    return ok;
 }
 // After a give-up: wait, bounded, for work that is still in flight.
 __device__ __forceinline__ void wait_drain(unsigned long long *b, uint32_t parity, unsigned long long limit_ns) {
