@@ -46,8 +46,13 @@
 // their own row of A only.
 //
 // Every wait is bounded (kWaitNs, then SHC_ETIMEOUT in the status word): all
-// roles leave their loops, the copies and products in flight are waited for,
-// TMEM is freed and the kernel returns.
+// roles of all CTAs of the cluster leave their loops, and the kernel returns.
+// Whether it finished or gave up, no CTA ends before what can still reach it
+// has: the loading thread waits for its stages' products, or after a give-up
+// for the copies themselves, the product warps for their last products, and
+// the loading threads of a pair, whose copies all signal the leader, tell one
+// another how many blocks they issued, so that the one behind can issue the
+// copies that the other's barrier phases wait for.
 #include <cuda.h>
 
 #include "f8.cuh"
@@ -67,7 +72,6 @@ constexpr int kPieceBytes = 32 * 64;  // a warp's staging of 32 output rows x 64
 // take 216, the other four keep 72: 2 x 216 + 72 = 504.
 constexpr int kEpiRegs = 216, kOtherRegs = 72;
 constexpr unsigned long long kWaitNs = 4000000000ull;
-constexpr unsigned long long kSettleNs = 2000000ull;
 
 // BN output columns per tile; PAIR CTAs (a cluster of one or two) work on one
 // tile of PAIR x 128 rows.
@@ -117,16 +121,24 @@ struct Control {
         unsigned long long full, empty;  // an accumulator holds a block's sums; they have been read
     } acc[2][4];  // [half][buffer]
     unsigned long long slot_full[kSlots], slot_empty[kSlots];
-    unsigned long long drain[2];
+    unsigned long long drain[2];  // a product warp's products are done, all of them
+    unsigned long long met;       // the other CTA of the pair has written `issued`
     int4 slot[kSlots];  // what a slot's scales are for: first row of this CTA, end of rows, first column, blocks (see kLast)
     int4 joined;  // SPLIT: first row, rows and first column of the tile whose sums are in the ring
     uint32_t tmem;
+    uint32_t issued;  // blocks that the other CTA of the pair has issued copies for
     int abort;
 };
 constexpr int kLast = 256;  // added to a slot's blocks where they are the tile's last ones
 
 // ---------------------------------------------------------------- waits
 
+// To a shared address of another CTA of the cluster (or of this one).
+__device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t rank, uint32_t v) {
+    asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, %1;\n st.shared::cluster.u32 [a], %2;\n}" ::"r"(addr),
+                 "r"(rank), "r"(v)
+                 : "memory");
+}
 __device__ __forceinline__ bool bar_test(unsigned long long *b, uint32_t parity) {
     uint32_t ok;
     asm volatile(
@@ -136,8 +148,16 @@ __device__ __forceinline__ bool bar_test(unsigned long long *b, uint32_t parity)
         : "memory");
     return ok != 0;
 }
-// True when the phase completed, false after kWaitNs or once another warp gave
-// up.  The clock is read on every 256th try only: reading it takes longer than
+// Ends the waits of every CTA of the cluster (of this one, where there is none).
+__device__ __forceinline__ void give_up(volatile int *abort, int *status) {
+    uint32_t n;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+#pragma unroll 1
+    for (uint32_t r = 0; r < n; r++) st_cluster(smem_u32(const_cast<const int *>(abort)), r, 1);
+    set_status(status, SHC_ETIMEOUT);
+}
+// True when the phase completed, false after kWaitNs or once a warp of the
+// cluster gave up.  The clock is read on every 256th try only: reading it takes longer than
 // most waits.  (Inline: a call would spill the epilogue's sums.)
 __device__ __forceinline__ bool bar_wait(unsigned long long *b, uint32_t parity, volatile int *abort, int *status) {
     unsigned long long t0 = 0;
@@ -149,8 +169,7 @@ __device__ __forceinline__ bool bar_wait(unsigned long long *b, uint32_t parity,
         const unsigned long long t = global_ns();
         if (t0 == 0) t0 = t;
         if (t - t0 > kWaitNs) {
-            *abort = 1;
-            set_status(status, SHC_ETIMEOUT);
+            give_up(abort, status);
             return false;
         }
     }
@@ -174,10 +193,10 @@ __device__ __forceinline__ bool warp_wait(unsigned long long *b, uint32_t parity
     __syncwarp();
     return ok;
 }
-// After a give-up: wait, bounded, for work that is still in flight.
-__device__ __forceinline__ void wait_drain(unsigned long long *b, uint32_t parity, unsigned long long limit_ns) {
+// For work in flight, which ends whether or not the kernel gave up: bounded by time alone.
+__device__ __forceinline__ void wait_drain(unsigned long long *b, uint32_t parity) {
     const unsigned long long t0 = global_ns();
-    while (!bar_test(b, parity) && global_ns() - t0 < limit_ns) {
+    while (!bar_test(b, parity) && global_ns() - t0 < kWaitNs) {
     }
 }
 __device__ __forceinline__ void expect_tx(unsigned long long *b, uint32_t bytes) {
@@ -257,6 +276,25 @@ template <int PAIR>
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
     if (PAIR == 2) asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
     else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// The loading threads of a pair meet, each once, and tell one another how many
+// blocks they have issued copies for.  Returns the other's (0 if it did not come).
+__device__ __forceinline__ uint32_t meet(Control &ctl, uint32_t rank, uint32_t issued) {
+    st_cluster(smem_u32(&ctl.issued), rank ^ 1, issued);
+    asm volatile(
+        "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, %1;\n mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n}" ::"r"(
+            smem_u32(&ctl.met)),
+        "r"(rank ^ 1)
+        : "memory");
+    uint32_t ok = 0;
+    const unsigned long long t0 = global_ns();
+    while (!ok && global_ns() - t0 < kWaitNs)
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], 0;\n selp.u32 %0, 1, 0, p;\n}"
+            : "=r"(ok)
+            : "r"(smem_u32(&ctl.met))
+            : "memory");
+    return ok ? *reinterpret_cast<volatile uint32_t *>(&ctl.issued) : 0;
 }
 template <bool CLUSTER>
 __device__ __forceinline__ void sync_all() {
@@ -558,6 +596,7 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1)
             mbar_init(&ctl.slot_empty[i], S::kEpiWarps);
         }
         for (int i = 0; i < 2; i++) mbar_init(&ctl.drain[i], 1);
+        mbar_init(&ctl.met, 1);
         ctl.abort = 0;
         ctl.joined = make_int4(0, 0, 0, 0);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -588,9 +627,11 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1)
         Tile tile;
         if (warp == S::kEpiWarps) {
             // ------------------------------------------------ loads
-            uint32_t it = 0;
-            bool ok = true;
-            while (ok && tiles.next(tile)) {
+            struct Boxes {
+                int mine;        // boxes of A for this CTA
+                uint32_t bytes;  // of a block, both CTAs'
+            };
+            const auto boxes_of = [&](const Tile &tile) {
                 int boxes[PAIR];  // of A, for each CTA
 #pragma unroll
                 for (int r = 0; r < PAIR; r++) {
@@ -598,10 +639,28 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1)
                     rows = rows < 0 ? 0 : rows > kTileM ? kTileM : rows;
                     boxes[r] = (rows + p.a_box - 1) / p.a_box;
                 }
-                const int mine = PAIR == 2 && rank ? boxes[PAIR - 1] : boxes[0];
-                uint32_t bytes = 0;
+                Boxes b{PAIR == 2 && rank ? boxes[PAIR - 1] : boxes[0], 0};
 #pragma unroll
-                for (int r = 0; r < PAIR; r++) bytes += boxes[r] * p.a_box * kTileK + S::kBBytes;
+                for (int r = 0; r < PAIR; r++) b.bytes += boxes[r] * p.a_box * kTileK + S::kBBytes;
+                return b;
+            };
+            const auto issue = [&](const Tile &tile, const Boxes &boxes, uint32_t s, int c) {
+                const uint32_t a = ring + s * S::kStageBytes, b = a + S::kABytes;
+                uint32_t bar = smem_u32(&ctl.full[s]);
+                if (rank == 0) expect_tx(&ctl.full[s], boxes.bytes);  // the leader counts both CTAs' bytes
+                if (PAIR == 2) bar = in_leader(bar);
+                for (int i = 0; i < boxes.mine; i++)
+                    tma_2d<PAIR>(a + i * p.a_box * kTileK, &map_a, bar, c * kTileK, tile.row0 + rank * kTileM + i * p.a_box);
+#pragma unroll
+                for (int j = 0; j < S::kBRows / 128; j++) {
+                    const int o = tile.col0 + rank * S::kBRows + j * 128, x = c * kTileK;
+                    tma_3d<PAIR>(b + j * 128 * kTileK, &map_w, bar, TRANS ? o : x, TRANS ? x : o, tile.expert);
+                }
+            };
+            uint32_t it = 0;
+            bool ok = true;
+            while (ok && tiles.next(tile)) {
+                const Boxes boxes = boxes_of(tile);
                 if (elect_one()) {
                     for (int c = c_begin; c < c_begin + blocks; c++) {
                         const uint32_t s = it % S::kStages, round = it / S::kStages;
@@ -609,30 +668,41 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1)
                             ok = false;
                             break;
                         }
-                        const uint32_t a = ring + s * S::kStageBytes, b = a + S::kABytes;
-                        uint32_t bar = smem_u32(&ctl.full[s]);
-                        if (rank == 0) expect_tx(&ctl.full[s], bytes);  // the leader counts both CTAs' bytes
-                        if (PAIR == 2) bar = in_leader(bar);
-                        for (int i = 0; i < mine; i++)
-                            tma_2d<PAIR>(a + i * p.a_box * kTileK, &map_a, bar, c * kTileK,
-                                         tile.row0 + rank * kTileM + i * p.a_box);
-#pragma unroll
-                        for (int j = 0; j < S::kBRows / 128; j++) {
-                            const int o = tile.col0 + rank * S::kBRows + j * 128, x = c * kTileK;
-                            tma_3d<PAIR>(b + j * 128 * kTileK, &map_w, bar, TRANS ? o : x, TRANS ? x : o, tile.expert);
-                        }
+                        issue(tile, boxes, s, c);
                         it++;
                     }
                 }
                 ok = __all_sync(~0u, (int)ok);
             }
+            // From here on to the end of what is in flight for this CTA.
             it = __reduce_max_sync(~0u, it);
-            if (lane == 0 && !ok) {  // copies still in flight land before the CTA ends
-                if (rank == 0)
-                    for (uint32_t k = it > S::kStages ? it - S::kStages : 0; k < it; k++)
-                        wait_drain(&ctl.full[k % S::kStages], (k / S::kStages) & 1, kWaitNs);
-                else  // these signal the other CTA's barriers
-                    wait_drain(&ctl.drain[0], 0, kSettleNs);
+            if (PAIR == 2) {
+                uint32_t other = 0;
+                if (elect_one()) other = meet(ctl, rank, it);
+                other = __reduce_max_sync(~0u, other);
+                if (it < other) {
+                    // After a give-up: the other CTA has loaded into stages, so they were free in both, and the
+                    // copies that complete their phases can be issued without a wait.
+                    Tiles<BN, PAIR> again(p);
+                    for (uint32_t k = 0; k < other && again.next(tile); k += blocks) {
+                        const Boxes boxes = boxes_of(tile);
+                        if (elect_one())
+                            for (uint32_t c = k < it ? it - k : 0; c < (uint32_t)blocks && k + c < other; c++)
+                                issue(tile, boxes, (k + c) % S::kStages, (int)c);
+                    }
+                    it = other;
+                }
+            }
+            if (elect_one()) {
+                const uint32_t last = it > S::kStages ? it - S::kStages : 0;
+                for (uint32_t k = last; k < it && ok; k++)
+                    ok = bar_wait(&ctl.done[k % S::kStages], (k / S::kStages) & 1, abort, p.status);
+                if (rank == 0) {
+                    for (uint32_t k = last; k < it && !ok; k++) wait_drain(&ctl.full[k % S::kStages], (k / S::kStages) & 1);
+                } else {  // its copies signal the leader, which waits for them; the leader's products signal here
+                    wait_drain(&ctl.drain[0], 0);
+                    wait_drain(&ctl.drain[1], 0);
+                }
             }
         } else if (warp < S::kEpiWarps + 3) {
             // ------------------------------------------------ products (of a pair: issued by its leader)
@@ -680,9 +750,9 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1)
                 first = (first + blocks) & 1;
                 ok = __all_sync(~0u, (int)ok);
             }
-            if (rank == 0 && !ok && elect_one()) {  // products still in flight end before TMEM is freed
+            if (rank == 0 && elect_one()) {  // its products end before TMEM is freed
                 mma_commit<PAIR>(&ctl.drain[me]);
-                wait_drain(&ctl.drain[me], 0, kWaitNs);
+                wait_drain(&ctl.drain[me], 0);
             }
         } else {
             // ------------------------------------------------ tiles and their scales for the epilogue
