@@ -218,8 +218,10 @@ int shc_decode_f8(shc_ctx *ctx, uint32_t dst_type, const uint8_t *codes, int64_t
  *                 A W^T's result as A, the gradient of its rows
  * A is encoded with block_rows 1; its scales are a_scale_stride apart from
  * row to row.  Each block's 128 products are summed in f32 and scaled by the
- * f32 product of the two scales; blocks are summed in f32, in an order that
- * the sizes alone decide, and the sum is rounded once to dst_type (SHC_SRC_*). */
+ * product of the two scales, rounded to f32's 24 bits also where it lies
+ * outside f32's range and the result does not; blocks are summed in f32, in an
+ * order that the sizes alone decide, and the sum is rounded once to dst_type
+ * (SHC_SRC_*). */
 int shc_matmul_f8(shc_ctx *ctx, const uint8_t *a, int64_t a_row_stride, const float *a_scales, int64_t a_scale_stride,
                   int64_t n_rows, const uint8_t *w, int64_t w_row_stride, const float *w_scales, int64_t n, int64_t k,
                   int transposed, uint32_t dst_type, void *dst, int64_t dst_row_stride, void *stream);

@@ -21,11 +21,14 @@
 #include <ucontext.h>
 #include <unistd.h>
 
+#include <math.h>
+
 #include <deque>
 #include <functional>
 #include <map>
 #include <random>
 #include <string>
+#include <type_traits>
 #include <vector>
 
 #define __device__
@@ -36,8 +39,9 @@ struct float2 { float x, y; };
 static int4 make_int4(int x, int y, int z, int w) { return {x, y, z, w}; }
 static float2 make_float2(float x, float y) { return {x, y}; }
 static float __uint_as_float(uint32_t u) { float f; memcpy(&f, &u, 4); return f; }
-static uint32_t as_uint(float f) { uint32_t u; memcpy(&u, &f, 4); return u; }
+static uint32_t __float_as_uint(float f) { uint32_t u; memcpy(&u, &f, 4); return u; }
 static float2 __ffma2_rn(float2 a, float2 b, float2 c) { return {a.x * b.x + c.x, a.y * b.y + c.y}; }
+static float2 __fmul2_rn(float2 a, float2 b) { return {a.x * b.x, a.y * b.y}; }
 static float __ldg(const float *p) { return *p; }
 static int __all_sync(unsigned, int v) { return v; }
 static unsigned __reduce_max_sync(unsigned, unsigned v) { return v; }
@@ -216,6 +220,7 @@ static void tma_3d(uint32_t dst, const CUtensorMap *m, uint32_t bar, int x, int 
 }
 
 #include "desc.inc"
+#include "scales.inc"
 
 static Tag operand(Cta &c, uint64_t desc) {
     const uint32_t at = (uint32_t)(desc & 0x3FFF) << 4;
@@ -312,12 +317,15 @@ static void mma_commit(unsigned long long *b) {
 static void fence_before() {}
 static void fence_after() {}
 
-static float value(const Sum &s, int c) { return (float)(1 + (c * 7 + s.row0 / 32 * 3 + s.col0 / 64 * 5 + s.expert) % 31); }
+// Sums are whole numbers times g_unit, scales whole numbers times powers of two,
+// so that everything is exact: in f32's range, and with products of scales below and above it.
+static float g_unit = 1.0f;
+static float value(const Sum &s, int c) { return g_unit * (float)(1 + (c * 7 + s.row0 / 32 * 3 + s.col0 / 64 * 5 + s.expert) % 31); }
 static void tmem_ld16(uint32_t addr, uint32_t r[16]) {
     const uint32_t d = (addr & 0xFFFF) / 128 * 128;
     const Sum s = here().tmem[d];
     check(s.steps == 4 && !here().waiting[d], "sums read while they are made");
-    for (int i = 0; i < 16; i++) r[i] = as_uint(value(s, s.c));
+    for (int i = 0; i < 16; i++) r[i] = __float_as_uint(value(s, s.c));
     yield();
 }
 static void tmem_wait_ld(uint32_t *) {}
@@ -333,12 +341,12 @@ static float wanted(int row, int col, int c0, int c1, int pair_rows) {
     (void)row0;
     Sum s;
     s.row0 = t->row0, s.col0 = t->col0, s.expert = t->expert;
-    float v = 0;
+    double v = 0;
     for (int c = c0; c < c1; c++)
-        v += value(s, c) * (g_sa[(size_t)row * g_args->a_scale_stride + c] *
+        v += (double)value(s, c) * ((double)g_sa[(size_t)row * g_args->a_scale_stride + c] *
                             g_sb[t->expert * g_args->w_scale_expert + (col < g_args->out ? col / 128 : t->col0 / 128) * g_args->w_scale_out +
                                  c * g_args->w_scale_in]);
-    return v;
+    return (float)v;
 }
 static int g_tm;  // rows of a tile
 template <int DT>
@@ -431,6 +439,10 @@ static void play(bool fault) {
     g_sb.resize((size_t)p.n_experts * nb * p.blocks_c);
     for (float &v : g_sa) v = (float)(1 + pick(4));
     for (float &v : g_sb) v = (float)(1 + pick(4));
+    const int range = (int)pick(3);  // the product of two scales: an ordinary number, a subnormal one, an infinite one
+    g_unit = range == 2 ? 0x1p-18f : 1.0f;
+    for (float &v : g_sa) v = ldexpf(v, range == 1 ? -80 : range == 2 ? 68 : 0);
+    for (float &v : g_sb) v = ldexpf(v, range == 1 ? -60 : range == 2 ? 60 : 0);
     p.a_scales = g_sa.data(), p.w_scales = g_sb.data();
     const int types[] = {SHC_SRC_F32, SHC_SRC_F16, SHC_SRC_BF16};
     p.dst_type = types[pick(3)];

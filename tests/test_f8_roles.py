@@ -29,6 +29,7 @@ def build(folder, text):
     parts = {
         "structs": between(text, "constexpr int kTileM", "// ---------------------------------------------------------------- waits"),
         "desc": between(text, "__device__ __forceinline__ uint64_t smem_desc", "template <int PAIR>\n__device__ __forceinline__ void mma_f8"),
+        "scales": between(text, "__device__ __forceinline__ void look(", "// ---------------------------------------------------------------- kernel"),
         "init": between(text, "    if (threadIdx.x == 0) {\n        for (int s = 0; s < S::kStages; s++) {", "    if (warp == S::kEpiWarps) {"),
         "roles": between(text, "    if (warp >= S::kEpiWarps) {\n        asm volatile(\"setmaxnreg", "    __syncwarp();\n    if (SPLIT) {"),
     }
