@@ -1100,7 +1100,7 @@ Plan plan_for(const MmArgs &a, int num_sms) {
         if (time < least) least = time, best = plan;
     };
     offer(350 + waves(128, 256, num_sms) * (200 + 47 * c), Plan{256, 1, 1});
-    offer(300 + waves(256, 256, num_sms / 2) * (340 + 41 * c), Plan{256, 2, 1});
+    if (num_sms >= 2) offer(300 + waves(256, 256, num_sms / 2) * (340 + 41 * c), Plan{256, 2, 1});
     const int64_t tiles = most_tiles(a, kTileM, 128), each = a.n_rows / a.n_experts, rows = each < kTileM ? each : kTileM;
     for (int z = 2; z <= 8; z *= 2) {
         if (tiles * z > (z == 8 ? 64 : num_sms) || c < 2 * z) break;
