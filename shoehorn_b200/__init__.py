@@ -363,14 +363,16 @@ class Context:
 
     def encode_f8(self, src, block_rows=1, out=None, scales=None, stream=None, sync=False):
         """Encode a [rows, cols] or [matrices, rows, cols] CUDA tensor
-        (bf16/f16/f32, adjacent columns, any other strides) to 8-bit blocks.
+        (bf16/f16/f32, or int16/uint16 as BF16 bits; adjacent columns, any other
+        strides) to 8-bit blocks.
 
         Returns (codes, scales): codes float8_e4m3fn of src's shape, each row
         on a 16-byte boundary; scales float32 [.., ceil(rows / block_rows),
         ceil(cols / 128)]."""
         torch = self.torch
         self._f8_here(src, "src")
-        st = self._f8_dtype(src.dtype)
+        dtype = src.dtype
+        st = SRC_BF16 if dtype is torch.int16 or dtype is torch.uint16 else self._f8_dtype(dtype)
         shape, stride = src.shape, src.stride()
         if len(shape) not in (2, 3):
             raise ValueError("src must have 2 or 3 dimensions")
