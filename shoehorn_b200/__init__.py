@@ -568,21 +568,23 @@ def _host_ptr(out):
     return ctypes.c_void_p(out.data_ptr())
 
 
-_default_ctx = None
+_default_ctxs = {}  # device: context
+_torch = None       # the module, once a default context was asked for
 
 
 def default_context(device=None):
     """Process-wide context on the current CUDA device (like the reference's
-    process-wide OnceLock grids)."""
-    global _default_ctx
-    ctx = _default_ctx
+    process-wide OnceLock grids).  Each device has its own, kept to the end:
+    captured graphs hold its status word."""
+    global _torch
+    if device is None:
+        if _torch is None:
+            import torch as _torch
+        device = _torch.cuda.current_device()
+    ctx = _default_ctxs.get(device)
     if ctx is None:
-        import torch
-    else:
-        torch = ctx.torch
-    dev = torch.cuda.current_device() if device is None else device
-    if ctx is None or ctx.device != dev:
-        ctx = _default_ctx = Context(dev)
+        ctx = Context(device)
+        ctx = _default_ctxs.setdefault(device, ctx)
     return ctx
 
 
