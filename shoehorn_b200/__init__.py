@@ -274,7 +274,12 @@ class Context:
     # weights), value = code * scale; include/shoehorn_cuda.h has the rules.
     # Every tensor has to be on the context's device.  Work goes to `stream`
     # (default: torch's current stream of that device); inputs have to be
-    # ready there, and results made here belong to it.
+    # ready there, and results made here belong to it.  Nothing is recorded for
+    # autograd, whatever the inputs require: codes have no gradient, and that
+    # of a product's rows is another product (transposed).  A kernel whose
+    # waits run out leaves its result unfinished; as for the other kernels, the
+    # context's sync raises that (torch's own synchronisation does not), and a
+    # captured graph needs its context to stay open.
     # Single-token calls are bound by the host, so each tensor's size, strides
     # and device are asked for once.
 
@@ -495,7 +500,9 @@ class Context:
         weight w [n, k] (block_rows 128), as [rows, n] of `dtype` (default
         bfloat16).  transposed: A W with a [rows, n], as [rows, k] (the
         gradient of the rows, given the encoded gradient of the product).
-        Sums are f32, rounded once."""
+        Sums are f32, rounded once; the two scales of a block may multiply to a
+        number outside f32's range where the result lies inside.  No gradient
+        is recorded."""
         return self._f8_product(a, a_scales, w, w_scales, None, bool(transposed), dtype, out, stream, sync)
 
     def matmul_f8_grouped(self, a, a_scales, w, w_scales, offsets, transposed=False, dtype=None, out=None, stream=None,

@@ -10,12 +10,14 @@
 // x / scale.  NaN and infinite elements become the NaN code and leave the
 // block's scale to the finite ones.
 //
-// All three kernels are bound by HBM: an element is read once and its code
-// written once (the tile kernel holds its tile in registers between the
-// maximum and the codes).  8192 x 14336 bf16 to 1 x 128 blocks 63.2 us (5.63
+// An element is read once and its code written once (the tile kernel holds its
+// tile in registers between the maximum and the codes); with rows on 16-byte
+// boundaries all three kernels are bound by HBM.  8192 x 14336 bf16 to 1 x 128 blocks 63.2 us (5.63
 // TB/s, 0.86 of the measured copy), to tiles 60.8, f32 87-91 us (6.5-6.8
 // TB/s); 14336 x 4096 tiles decoded to bf16 28.6 us (6.16 TB/s, 0.94).  Rows
-// that start off 16-byte boundaries: 8192 x 14330 bf16 97 us, f32 101.
+// that start off 16-byte boundaries take longer (8192 x 14330 bf16 97 us, 0.55
+// of the copy; f32 101; 4096 x 14331 decoded to bf16 45.8), by what was not
+// profiled.
 #include "f8.cuh"
 
 namespace shc {

@@ -33,10 +33,10 @@
 // SMs idle, a cluster shares a tile's contraction and joins its sums through
 // distributed shared memory, in rank order: no atomics, no workspace.
 //
-// What bounds it (4096 x 14336 x 4096, a pair's 256 x 256 tiles, 221-250 us,
-// 1.93-2.18 PFLOP/s, with the clock that the power limit leaves): the
-// products alone take 138 us (514 cycles a block, their rate), the loads
-// alone 113 us (17 TB/s from L2), but a block passes in 865 cycles, because
+// What bounds it (4096 x 14336 x 4096, a pair's 256 x 256 tiles, 218-253 us,
+// 1.90-2.21 PFLOP/s, with the clock that the power limit leaves; the parts were
+// timed where the whole took 227): the products alone take 138 us (514 cycles
+// a block, their rate), the loads alone 113 us (17 TB/s from L2), but a block passes in 865 cycles, because
 // an epilogue warp needs that long to wait for, read and scale its 128
 // columns.  With one multiply-add in eight it took 202 us, without the stores
 // 217, without either 164 (where the whole took 227).  Sixteen
@@ -44,9 +44,10 @@
 // loads 290 (spilled), a single warp issuing products and acknowledging on
 // two barriers a block 301.
 //
-// Rows of an expert (or of the whole matrix) that lie past its end are loaded
-// as zeros or as the next expert's rows, and not stored: rows of D depend on
-// their own row of A only.
+// Rows of a tile that lie past the end of their expert (or of the whole
+// matrix) are loaded as zeros or as the next expert's rows, or, behind the last
+// box that holds a row, not at all (the stage keeps what was there).  They are
+// not stored: rows of D depend on their own row of A only.
 //
 // Every wait is bounded (kWaitNs, then SHC_ETIMEOUT in the status word): all
 // roles of all CTAs of the cluster leave their loops, and the kernel returns.
@@ -897,7 +898,7 @@ __global__ void __launch_bounds__(Shape<BN, PAIR>::kThreads, 1)
             }
             // The slot's blocks; with_twos: their sums are multiplied by powers of two first.  (Two loops: the
             // choice within one took the prompt's product from 236 to 252 us.  All-zero blocks have the least
-            // scale and come here too: 96 zero rows among 4096 take 5 % more, zero rows in every tile 47 %.)
+            // scale and come here too: 93 zero rows among 4096 take 5 % more, a zero row in every tile half as much again.)
             const auto blocks_of_slot = [&](auto with_twos) {
                 constexpr bool kTwos = decltype(with_twos)::value;
                 const float *scales = slots + slot * (S::kSlotBytes / 4) + lanes0 + lane;
@@ -1066,20 +1067,26 @@ int64_t most_tiles(const MmArgs &a, int tm, int bn) {
 
 // Which tiles to use: the least of the times below, in units of 10 ns, fitted
 // to 60 products of 1 to 8192 rows, 1024 to 14336 columns and 8 to 112 blocks
-// (within 15 % of all but those that HBM bounds, where the shapes tie).
+// with 16-bit results in rows on 16-byte boundaries (within 20 % of all but
+// those that HBM bounds, where the shapes tie).  It knows neither wider results
+// nor rows off those boundaries nor how many experts have rows, and is off
+// there: 7.5 us for 1037 x 2008 x 1030 to f32 (9.7-11.9 measured), 15.0 for the
+// gradient of 3001 rows and 16 experts, 1000 x 2050 to f32 (24-32), 242 for 4096
+// rows of 8 uneven experts, 14336 x 4096 (270-330), 27.1 for 96 rows over 64
+// experts, 2048 x 1024 (23).
 //
 //   tile                    start   each wave of tiles        4096 cubed, measured
 //   128 x 128               3.9 us  1.0 us + 0.29 x blocks    79 us
 //   128 x 256               3.5     2.0    + 0.47             71
-//   256 x 256, CTA pair     3.0     3.4    + 0.41             68
+//   256 x 256, CTA pair     3.0     3.4    + 0.41             70
 //
 // A grouped product has row tiles for whole tiles' rows and half a tile more
 // for each expert, or one for each expert with rows.  Where 128 x 128 tiles
-// leave most SMs idle, a cluster of CTAs shares a tile's contraction: joining
-// two parts takes 1.7 us + 3.5 x rows / 128 and four or eight 1.3 + 2.8 x rows
-// / 128, whatever the number of blocks, so that one row through 4096 x 4096
-// takes 8.7 us in four parts (13.2 in one) and 128 rows through 2048 x 1024 6.1
-// in one (8.1 in four).  Clusters of eight do not all run at once beyond 64
+// leave most SMs idle, a cluster of CTAs shares a tile's contraction: 4.9 us + 0.29
+// x a part's blocks, and joining two parts takes 1.7 us + 3.5 x rows / 128 and
+// four or eight 1.3 + 2.8 x rows / 128, whatever the number of blocks, so that
+// one row through 4096 x 4096 takes 8.8 us in four parts (13.2 in one) and 128
+// rows through 2048 x 1024 6.1 in one (8.1 in four).  Clusters of eight do not all run at once beyond 64
 // CTAs (16 of them take twice as long as 8).
 struct Plan {
     int bn, pair, split;
